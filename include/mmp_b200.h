@@ -135,6 +135,23 @@ int mmp_rope_kv_write(const void* q, int64_t q_b, const void* k, int64_t k_b, co
                       int block_size, int num_blocks, const int64_t* slot_mapping,
                       int batch, int* err, void* stream);
 
+/* ---- RoPE with several position axes + key multiplier + paged KV write ---------------------------------
+ * The several-axis form of mmp_rope_kv_write (no counterpart in the reference, whose positions have one axis): tokens of
+ * images and video carry a position for each axis (time, height, width). qkv: [T, (nq + 2 nkv) hd] bf16 rows [q | k | v]
+ * with row stride `row`. Pair i < rd / 2 of a head (dims i and i + rd / 2; dims >= rd are not rotated) of q and of
+ * key_mult * k turns by positions[axes[i], t] * inv_freq[i], the product taken exactly (far positions keep their angle).
+ * positions: [naxes, T] int64, rows of stride p_a; inv_freq, axes: [rd / 2] fp32 / int32 (an axis outside [0, naxes) sets
+ * MMP_DEVERR_INDEX and counts as axis 0). q goes to q_out [T, nq hd] (row stride qo_b; may be the q part of qkv itself);
+ * key_mult * k, rotated, and v go to the caches at slot_mapping[t] (neither where it is < 0; a slot past the cache sets
+ * MMP_DEVERR_INDEX); caches as in mmp_rope_kv_write. Any hd <= 1024 and even rd <= hd; 16-byte accesses where rd / 2, hd and
+ * the rows are multiples of 8 values, single values otherwise. Slots must differ.
+ */
+int mmp_mrope_kv_write(const void* qkv, int64_t row, int nq, int nkv, int hd, const int64_t* positions, int64_t p_a,
+                       int naxes, const float* inv_freq, const int32_t* axes, int rd, float key_mult, void* q_out,
+                       int64_t qo_b, void* key_cache, void* value_cache, int64_t c_block, int64_t c_tok,
+                       int64_t c_head, int block_size, int num_blocks, const int64_t* slot_mapping, int T,
+                       int* err, void* stream);
+
 /* ---- SwiGLU activation ----------------------------------------------------------------------------
  * Replaces kernels.silu_and_mul (harness/kernels.py:31-37) and the MLP's `F.silu(g * gm) * u`
  * (harness/layer.py:135): out[r, c] = silu(gate_scale * gate[r, c]) * up[r, c], bf16, row strides in
@@ -355,6 +372,39 @@ int mmp_gdn_prefill_tc(const void* q, int64_t q_t, int64_t q_h, const void* k, i
                        void* out, int64_t o_t, int64_t o_h,
                        int nseq, int ntok, int nk, int nv, int dk, int dv, int lines,
                        void* workspace, size_t workspace_bytes, int* err, void* stream);
+
+/* ---- mixture of experts -----------------------------------------------------------------------------
+ * The reference only models the bytes of this layer for its Qwen3.5-A3B description (configs/qwen35_35b_a3b.yaml:1-22,
+ * harness/synth.py:114-138); its own MoE template (harness/seq_model.py:274-332) routes on the host.
+ *
+ * mmp_moe_route: l = logits[t, :E] in fp32 (NaN counts as -inf, +inf as the largest float). The top_k largest, falling,
+ * ties to the lowest index: ids[t, k] and weights[t, k] = exp(l_k - max) / Z, Z the sum over the chosen (renormalize) or
+ * over all experts. An expert at -inf is never chosen: places without an expert hold id -1 and weight 0. shared: one more
+ * place with id E and weight sigmoid(logits[t, E]) (the gate of an expert that every token takes). logits: fp32 or bf16
+ * rows of stride l_t; weights, ids: [T, top_k + shared], contiguous. E <= 1024, top_k + shared <= 32.
+ *
+ * mmp_moe_experts: out_t = addend_t + sum_k weights[t, k] * Wd_e (silu(Wg_e x_t) * (Wu_e x_t)), e = ids[t, k]; a place with
+ * id < 0 adds nothing, an id >= E sets MMP_DEVERR_INDEX and adds nothing, an expert twice in a row adds twice. x: [T, H]
+ * bf16; w_gate_up: [E, 2 I, H] bf16, an expert's I gate rows, then its I up rows (strides gu_e, gu_r); w_down: [E, H, I]
+ * bf16 (d_e, d_r); weights / ids: [T, places] with row strides; addend: [T, H] bf16 or NULL; out: [T, H] bf16, may be the
+ * addend. The products of the first are rounded to bf16 (silu * up, the second's operand), all sums are fp32. H and I
+ * multiples of 8, rows 16-byte aligned, places <= 32, E <= 1024, T * places <= 2^26. workspace: 256-byte aligned, at least
+ * mmp_moe_workspace_size(T, places, H, I, E) bytes, scratch of this call alone: calls that may overlap on the GPU, captured
+ * ones among them, need one each.
+ *
+ * mmp_moe_layer: both from the logits ([T, E], columns as mmp_moe_route takes them); with few tokens routing and the sort by expert are one
+ * launch. E counts the experts of the weight tensors, the shared one (their last) included. */
+int mmp_moe_route(const void* logits, int logits_dtype, int64_t l_t, int T, int E, int top_k, int renormalize, int shared,
+                  float* weights, int32_t* ids, void* stream);
+size_t mmp_moe_workspace_size(int T, int places, int H, int I, int E);
+int mmp_moe_experts(const void* x, int64_t x_t, const void* w_gate_up, int64_t gu_e, int64_t gu_r, const void* w_down,
+                    int64_t d_e, int64_t d_r, const float* weights, int64_t w_t, const int32_t* ids, int64_t id_t,
+                    const void* addend, int64_t a_t, void* out, int64_t o_t, int T, int places, int H, int I, int E,
+                    void* workspace, size_t workspace_bytes, int* err, void* stream);
+int mmp_moe_layer(const void* x, int64_t x_t, const void* logits, int logits_dtype, int64_t l_t, const void* w_gate_up,
+                  int64_t gu_e, int64_t gu_r, const void* w_down, int64_t d_e, int64_t d_r, const void* addend,
+                  int64_t a_t, void* out, int64_t o_t, int T, int top_k, int renormalize, int shared, int H, int I, int E,
+                  void* workspace, size_t workspace_bytes, int* err, void* stream);
 
 /* ---- peer-memory all-reduce fused with the residual add and RMSNorm (decode-sized messages) ------------
  * Replaces the NCCL all-reduce of the layer's partial sums (`ParallelHybridLayer._ar`, harness/layer.py:175-181)

@@ -34,6 +34,14 @@ SIGNATURES: dict[str, tuple] = {
     "mmp_gated_rmsnorm": (I32, [P, I64, P, I64, P, P, I64, P, I32, I32, I32, I32, F32, F32, P]),
     "mmp_rope_kv_write": (I32, [P, I64, P, I64, P, I64, I32, I32, I32, P, P, I32, P, F32, P, I64, P, I64,
                                 P, P, I64, I64, I64, I32, I32, P, I32, P, P]),
+    "mmp_mrope_kv_write": (I32, [P, I64, I32, I32, I32, P, I64, I32, P, P, I32, F32, P, I64, P, P, I64, I64, I64, I32,
+                                 I32, P, I32, P, P]),
+    "mmp_moe_route": (I32, [P, I32, I64, I32, I32, I32, I32, I32, P, P, P]),
+    "mmp_moe_workspace_size": (SZ, [I32, I32, I32, I32, I32]),
+    "mmp_moe_experts": (I32, [P, I64, P, I64, I64, P, I64, I64, P, I64, P, I64, P, I64, P, I64, I32, I32, I32, I32, I32,
+                              P, SZ, P, P]),
+    "mmp_moe_layer": (I32, [P, I64, P, I32, I64, P, I64, I64, P, I64, I64, P, I64, P, I64, I32, I32, I32, I32, I32, I32,
+                            I32, P, SZ, P, P]),
     "mmp_silu_mul": (I32, [P, I64, P, I64, P, I64, I32, I32, F32, P]),
     "mmp_paged_attn_workspace_size": (SZ, [I32, I32, I32, I32]),
     "mmp_paged_attn_decode": (I32, [P, I64, I64, P, P, I64, I64, I64, P, I64, P, P, I64, I64, I32, I32, I32, I32, I32,

@@ -8,6 +8,7 @@ buffers, epilogue scales, workspaces) expose the fusions the layer uses.
 """
 from __future__ import annotations
 
+import contextlib
 import math
 
 import torch
@@ -49,6 +50,23 @@ def _rowmajor(name: str, t: torch.Tensor) -> int:
         raise ValueError(f"{name}: expected a 2-D tensor with a contiguous last dimension, got {tuple(t.shape)} "
                          f"strides {t.stride()}")
     return t.stride(0)
+
+
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def _on(t: torch.Tensor):
+    """The device of t as the current one (the library launches on the current device)."""
+    if not t.is_cuda or t.device.index == torch.cuda.current_device():
+        return _NO_SWITCH
+    return torch.cuda.device(t.device)
+
+
+def _one_device(name: str, *ts: torch.Tensor | None) -> None:
+    _cuda(name, *ts)
+    devs = {t.device for t in ts if t is not None}
+    if len(devs) > 1:
+        raise ValueError(f"{name}: tensors on several devices: {sorted(map(str, devs))}")
 
 
 def error_word(device: torch.device) -> torch.Tensor:
@@ -242,6 +260,60 @@ def qkv_rope_kv_write(qkv: torch.Tensor, nq: int, nkv: int, head_dim: int, posit
               nq, nkv, head_dim, _p(positions), None, 0, _p(inv_freq), float(key_mult),
               _p(q_out), _rowmajor("q_out", q_out), None, 0, _p(key_cache), _p(value_cache), cb, ct, ch, blk, nb,
               _p(slot_mapping), T, _p(error_word(qkv.device)), _stream(qkv))
+    return q_out
+
+
+def rope_axes(sections, interleaved: bool, device: torch.device) -> torch.Tensor:
+    """[sum(sections)] int32: the position axis of every rotated pair. sections[a] pairs turn with axis a. In blocks: the
+    first sections[0] pairs axis 0, the next sections[1] axis 1, and so on. Interleaved over n axes: pair i has axis i mod n
+    while i < n * sections[i mod n], axis 0 otherwise."""
+    sec = [int(s) for s in sections]
+    if not sec or any(s < 0 for s in sec) or sum(sec) == 0:
+        raise ValueError(f"rope_axes: sections {sections} must be non-negative with a positive sum")
+    n, half = len(sec), sum(sec)
+    if interleaved:
+        ax = [i % n if i < n * sec[i % n] else 0 for i in range(half)]
+        if any(ax.count(a) != sec[a] for a in range(n)):
+            raise ValueError(f"rope_axes: sections {sections} do not interleave (axis a needs n * sections[a] <= the pairs)")
+    else:
+        ax = [a for a in range(n) for _ in range(sec[a])]
+    return torch.tensor(ax, dtype=torch.int32).to(device)
+
+
+def qkv_mrope_kv_write(qkv: torch.Tensor, nq: int, nkv: int, head_dim: int, positions: torch.Tensor,
+                       inv_freq: torch.Tensor, axes: torch.Tensor, key_mult: float, q_out: torch.Tensor,
+                       key_cache: torch.Tensor, value_cache: torch.Tensor, slot_mapping: torch.Tensor) -> torch.Tensor:
+    """qkv_rope_kv_write for positions with several axes (time, height, width): positions [naxes, T] int64; pair i of a head
+    (dims i and i + rd/2, rd = 2 * inv_freq.numel() <= head_dim; the dims from rd on pass unrotated) turns by
+    positions[axes[i], t] * inv_freq[i] (axes from rope_axes). Rows with slot_mapping < 0 are rotated into q_out and not
+    cached. Angles are exact at any position."""
+    name = "qkv_mrope_kv_write"
+    _one_device(name, qkv, positions, inv_freq, axes, q_out, key_cache, value_cache, slot_mapping)
+    for t in (qkv, q_out, key_cache, value_cache):
+        _dtype(name, t, BF16)
+    for t in (positions, slot_mapping):
+        _dtype(name, t, torch.int64)
+    _dtype(name, inv_freq, torch.float32)
+    _dtype(name, axes, torch.int32)
+    T = qkv.shape[0]
+    if qkv.dim() != 2 or qkv.shape[1] != (nq + 2 * nkv) * head_dim:
+        raise ValueError(f"{name}: qkv {tuple(qkv.shape)} is not [T, ({nq} + 2 * {nkv}) * {head_dim}]")
+    if positions.dim() != 2 or positions.shape[1] != T or (T > 1 and positions.stride(1) != 1):
+        raise ValueError(f"{name}: positions must be [axes, {T}] with contiguous rows, got {tuple(positions.shape)}")
+    if inv_freq.dim() != 1 or inv_freq.shape != axes.shape or not inv_freq.is_contiguous() or not axes.is_contiguous():
+        raise ValueError(f"{name}: inv_freq and axes must be contiguous vectors of one length")
+    if slot_mapping.shape != (T,) or (T > 1 and slot_mapping.stride(0) != 1):
+        raise ValueError(f"{name}: slot_mapping must be a contiguous [{T}]")
+    if q_out.shape != (T, nq * head_dim):
+        raise ValueError(f"{name}: q_out {tuple(q_out.shape)} is not [{T}, {nq * head_dim}]")
+    cb, ct, ch, blk, nb = _cache_strides(key_cache, value_cache)
+    if key_cache.shape != value_cache.shape or key_cache.shape[2:] != (nkv, head_dim):
+        raise ValueError(f"{name}: caches {tuple(key_cache.shape)} are not [blocks, block, {nkv}, {head_dim}]")
+    with _on(qkv):
+        _lib.call("mmp_mrope_kv_write", _p(qkv), _rowmajor("qkv", qkv), nq, nkv, head_dim, _p(positions),
+                  positions.stride(0), positions.shape[0], _p(inv_freq), _p(axes), 2 * inv_freq.shape[0], float(key_mult),
+                  _p(q_out), _rowmajor("q_out", q_out), _p(key_cache), _p(value_cache), cb, ct, ch, blk, nb,
+                  _p(slot_mapping), T, _p(error_word(qkv.device)), _stream(qkv))
     return q_out
 
 
@@ -646,4 +718,122 @@ def gdn_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, a: torch.Tens
                   _p(error_word(q.device)), _stream(q), kernels=2)
     else:
         _lib.call("mmp_gdn_prefill", *args, _p(error_word(q.device)), _stream(q))
+    return out
+
+
+# ----------------------------------------------------------------------------- mixture of experts
+def _logits_dtype(name: str, logits: torch.Tensor) -> int:
+    if logits.dtype not in (torch.float32, BF16):
+        raise ValueError(f"{name}: logits must be fp32 or bf16, got {logits.dtype}")
+    return MMP_F32 if logits.dtype == torch.float32 else MMP_BF16
+
+
+def moe_route(logits: torch.Tensor, top_k: int, weights: torch.Tensor | None = None, ids: torch.Tensor | None = None,
+              renormalize: bool = True, shared: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """Top-k routing from the router's logits [T, E] (fp32 or bf16): weights fp32 and ids int32, both [T, top_k], by falling
+    logit, ties to the lowest index; weights are the softmax over the experts, over the chosen ones with renormalize. An
+    expert at -inf (or NaN) is never chosen; a place without an expert has id -1 and weight 0.
+    shared: logits is [T, E + 1] and one more place follows, id E with weight sigmoid(logits[:, E]): an expert that every
+    token takes, behind a gate of its own."""
+    name = "moe_route"
+    _one_device(name, logits, weights, ids)
+    dt, l_t = _logits_dtype(name, logits), _rowmajor("logits", logits)
+    T, n, places = logits.shape[0], logits.shape[1] - bool(shared), int(top_k) + bool(shared)
+    if weights is None:
+        weights = torch.empty(T, places, dtype=torch.float32, device=logits.device)
+    if ids is None:
+        ids = torch.empty(T, places, dtype=torch.int32, device=logits.device)
+    _dtype(name, weights, torch.float32)
+    _dtype(name, ids, torch.int32)
+    for nm, t in (("weights", weights), ("ids", ids)):
+        if t.shape != (T, places) or not t.is_contiguous():
+            raise ValueError(f"{name}: {nm} must be a contiguous [{T}, {places}], got {tuple(t.shape)}")
+    with _on(logits):
+        _lib.call("mmp_moe_route", _p(logits), dt, l_t, T, n, int(top_k), int(bool(renormalize)), int(bool(shared)),
+                  _p(weights), _p(ids), _stream(logits))
+    return weights, ids
+
+
+def moe_workspace(T: int, places: int, hidden: int, intermediate: int, experts: int, device: torch.device) -> torch.Tensor:
+    """Scratch for moe_experts / moe_layer of up to these sizes (places: ids per token, the shared expert's included).
+    Calls that may overlap on the GPU (two streams, two captured graphs) need one each."""
+    n = _lib.lib().mmp_moe_workspace_size(T, places, hidden, intermediate, experts)
+    return torch.empty(max(256, n), dtype=torch.uint8, device=device)
+
+
+def _moe_common(name: str, x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, addend: torch.Tensor | None,
+                out: torch.Tensor | None, workspace: torch.Tensor | None, places: int):
+    for t in (x, w_gate_up, w_down, addend, out):
+        _dtype(name, t, BF16)
+    if x.dim() != 2 or w_gate_up.dim() != 3 or w_down.dim() != 3:
+        raise ValueError(f"{name}: x [T, H], w_gate_up [E, 2 I, H] and w_down [E, H, I] expected")
+    T, H = x.shape
+    E, I = w_down.shape[0], w_down.shape[2]
+    if w_gate_up.shape != (E, 2 * I, H) or w_down.shape[1] != H:
+        raise ValueError(f"{name}: shapes disagree: x {tuple(x.shape)}, w_gate_up {tuple(w_gate_up.shape)}, "
+                         f"w_down {tuple(w_down.shape)}")
+    if w_gate_up.stride(2) != 1 or w_down.stride(2) != 1:
+        raise ValueError(f"{name}: the weights' last dimension must be contiguous")
+    if out is None:
+        out = torch.empty(T, H, dtype=BF16, device=x.device)
+    for nm, t in (("addend", addend), ("out", out)):
+        if t is not None and t.shape != (T, H):
+            raise ValueError(f"{name}: {nm} {tuple(t.shape)} is not [{T}, {H}]")
+    if workspace is None:
+        workspace = moe_workspace(T, places, H, I, E, x.device)
+    return T, H, I, E, out, workspace
+
+
+def _row(t: torch.Tensor | None, name: str) -> int:
+    """Row stride; of a single row, which has none, its length."""
+    if t is None:
+        return 0
+    s = _rowmajor(name, t)
+    return s if t.shape[0] > 1 else (t.shape[1] + 7) // 8 * 8
+
+
+def moe_experts(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, weights: torch.Tensor, ids: torch.Tensor,
+                out: torch.Tensor | None = None, addend: torch.Tensor | None = None,
+                workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """out[t] = addend[t] + sum_k weights[t, k] * (silu(x[t] Wg^T) * (x[t] Wu^T)) Wd^T with the expert ids[t, k]: x [T, H],
+    w_gate_up [E, 2 I, H] (gate rows, then up rows), w_down [E, H, I], all bf16; weights fp32 and ids int32 [T, places] (as
+    moe_route gives them). A place with id < 0 adds nothing; an id >= E is reported through the error word and adds nothing.
+    out may be the addend. workspace: moe_workspace; without one, scratch is allocated for this call."""
+    name = "moe_experts"
+    _one_device(name, x, w_gate_up, w_down, weights, ids, out, addend, workspace)
+    _dtype(name, weights, torch.float32)
+    _dtype(name, ids, torch.int32)
+    if ids.dim() != 2 or ids.shape[0] != x.shape[0] or weights.shape != ids.shape:
+        raise ValueError(f"{name}: weights and ids must be [{x.shape[0]}, places], got {tuple(weights.shape)} and {tuple(ids.shape)}")
+    T, H, I, E, out, ws = _moe_common(name, x, w_gate_up, w_down, addend, out, workspace, ids.shape[1])
+    with _on(x):
+        _lib.call("mmp_moe_experts", _p(x), _row(x, "x"), _p(w_gate_up), w_gate_up.stride(0), w_gate_up.stride(1), _p(w_down),
+                  w_down.stride(0), w_down.stride(1), _p(weights), _rowmajor("weights", weights), _p(ids),
+                  _rowmajor("ids", ids), _p(addend), _row(addend, "addend"), _p(out), _row(out, "out"), T, ids.shape[1],
+                  H, I, E, _p(ws), ws.numel() * ws.element_size(), _p(error_word(x.device)), _stream(x),
+                  kernels=0 if T == 0 else 3 if T * ids.shape[1] <= MOE_FEW_PLACES else 6)
+    return out
+
+
+MOE_FEW_PLACES = 1536  # tokens * places up to which the products stream weights without sorting through tensor memory
+
+
+def moe_layer(x: torch.Tensor, logits: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, top_k: int,
+              out: torch.Tensor | None = None, renormalize: bool = True, shared: bool = False,
+              addend: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """moe_route and moe_experts in one call: with few tokens, routing, sorting and both products are three launches. logits
+    [T, E] (shared: the same E columns, the last one the shared expert's gate; its weights are the last of w_gate_up and
+    w_down)."""
+    name = "moe_layer"
+    _one_device(name, x, logits, w_gate_up, w_down, out, addend, workspace)
+    dt, l_t, places = _logits_dtype(name, logits), _rowmajor("logits", logits), int(top_k) + bool(shared)
+    T, H, I, E, out, ws = _moe_common(name, x, w_gate_up, w_down, addend, out, workspace, places)
+    if logits.shape != (T, E):
+        raise ValueError(f"{name}: logits {tuple(logits.shape)} is not [{T}, {E}]")
+    with _on(x):
+        _lib.call("mmp_moe_layer", _p(x), _row(x, "x"), _p(logits), dt, l_t, _p(w_gate_up), w_gate_up.stride(0),
+                  w_gate_up.stride(1), _p(w_down), w_down.stride(0), w_down.stride(1), _p(addend), _row(addend, "addend"),
+                  _p(out), _row(out, "out"), T, int(top_k), int(bool(renormalize)), int(bool(shared)), H, I, E, _p(ws),
+                  ws.numel() * ws.element_size(), _p(error_word(x.device)), _stream(x),
+                  kernels=0 if T == 0 else 3 if T * places <= MOE_FEW_PLACES else 7)
     return out
