@@ -261,6 +261,18 @@ __global__ void __launch_bounds__(256) moe_scatter(const MoeArgs A) {
   }
 }
 
+// Each token's row to the sorted rows of its places: block (token), read once, written once a place.
+__global__ void __launch_bounds__(256) moe_sort_rows(const MoeArgs A) {
+  const int64_t t = blockIdx.x;
+  for (int c = threadIdx.x * 8; c < A.H; c += 256 * 8) {
+    const uint4 v = ld16(A.x + t * A.x_t + c);
+    for (int k = 0; k < A.places; ++k) {
+      const int r = A.pos[t * A.places + k];
+      if (r >= 0) st16(A.xs + static_cast<int64_t>(r) * A.H + c, v);
+    }
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ few-token products
 __device__ __forceinline__ void mma_16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                           uint32_t b1) {
@@ -553,6 +565,7 @@ int many_products(const MoeArgs& A, const MoeLayout& L, cudaStream_t s) {
   moe_count<<<L.chunks, 256, 0, s>>>(A);
   moe_scan<<<1, 1024, 0, s>>>(A, L.chunks);
   moe_scatter<<<L.chunks, 256, 0, s>>>(A);
+  moe_sort_rows<<<A.T, 256, 0, s>>>(A);
   int rc = mmp_check_launch("mmp_moe_experts");
   if (rc != MMP_OK) return rc;
   if ((rc = moe_products_tc(A, L.max_blocks, s)) != MMP_OK) return rc;
@@ -600,6 +613,7 @@ void place_workspace(MoeArgs& A, const MoeLayout& L, void* workspace) {
   A.rows = reinterpret_cast<int*>(w + L.rows);
   A.pos = reinterpret_cast<int*>(w + L.pos);
   A.counts = reinterpret_cast<int*>(w + L.counts);
+  A.xs = reinterpret_cast<bf16*>(w + L.xs);
   A.h = reinterpret_cast<bf16*>(w + L.h);
   A.y = reinterpret_cast<float*>(w + L.y);
 }

@@ -23,7 +23,7 @@ struct MoeHeader {
 
 // Workspace offsets in bytes, every part 256-byte aligned.
 struct MoeLayout {
-  size_t header, recs, blocks, rows, pos, weights, ids, counts, h, y, bytes;
+  size_t header, recs, blocks, rows, pos, weights, ids, counts, xs, h, y, bytes;
   int chunks, max_blocks;
 };
 
@@ -45,6 +45,7 @@ inline MoeLayout moe_layout(int64_t T, int places, int H, int I, int E) {
   L.weights = part(R * 4);
   L.ids = part(R * 4);
   L.counts = part(static_cast<size_t>(L.chunks) * E * 4);
+  L.xs = part(few ? 0 : R * H * 2);
   L.h = part(R * I * 2);
   L.y = part(few ? 0 : R * H * 4);
   L.bytes = at;
@@ -67,6 +68,7 @@ struct MoeArgs {
   int* rows;      // sorted row -> place
   int* pos;       // place -> sorted row, -1 where the place has no expert
   int* counts;    // [chunk][expert]
+  bf16* xs;       // [sorted row][H]: x in the order of the rows (tensor-core path)
   bf16* h;        // [sorted row][I]
   float* y;       // [sorted row][H]
   int* err;

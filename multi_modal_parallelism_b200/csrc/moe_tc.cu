@@ -5,8 +5,9 @@
 // in steps of 16) its N side: an expert's weights are read once for up to 256 tokens and little of an MMA is padding. Up to
 // about 250 rows an expert the layer is bound by reading the weights, above it by the MMAs.
 //   * up: the A tile is 64 gate and 64 up rows, alternating in groups of 8: one box of a 5-D tensor map over the
-//     [expert][gate | up][row] layout. Gate and up values of one column of h then sit 8 lanes apart in one warp. The token
-//     rows are gathered straight from x by TMA (four rows an instruction, the lanes of one warp issue them).
+//     [expert][gate | up][row] layout. Gate and up values of one column of h then sit 8 lanes apart in one warp. B are the
+//     expert's rows of xs, x sorted by a kernel before this one (gathered by TMA, four rows an instruction, the same kernel
+//     took four times as long: one such instruction every 66 clocks).
 //   * down: A is 128 rows of Wd, B the expert's consecutive rows of h. fp32 results per place go to y, and moe_combine sums
 //     each token's places in their order.
 // One persistent block an SM; warp 0 streams both operands through a ring of shared-memory stages across tiles, one lane of
@@ -37,13 +38,6 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map
       "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];\n"
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(u), "r"(v) : "memory");
 }
-// four rows of a 2-D map whose box is one row high
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int4 r) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];\n"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w) : "memory");
-}
-
 template <bool UP, int STAGES>
 __global__ void __launch_bounds__(MTHREADS, 1) moe_tc_kernel(const __grid_constant__ CUtensorMap tmA,
                                                              const __grid_constant__ CUtensorMap tmB, const MoeArgs A, int tiles) {
@@ -93,21 +87,9 @@ __global__ void __launch_bounds__(MTHREADS, 1) moe_tc_kernel(const __grid_consta
     for (int it = blockIdx.x; it < nitems && ok; it += gridDim.x) {
       const int4 blk = __ldcg(A.blocks + it / tiles);
       const int tile = it % tiles;
-      // B rows of a stage: up, in fours (this lane's rows 4 lane .. and 128 + 4 lane ..; rows past the block's last repeat
-      // it, their columns are not read); down, in boxes of 32 rows (rows past the block's are not read either)
-      const int nb = UP ? (blk.z + 3) / 4 : (blk.z + 31) / 32;
-      int4 r[2];
-      if constexpr (UP) {
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          int v[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            v[j] = __ldcg(A.rows + blk.y + min(q * 128 + lane * 4 + j, blk.z - 1)) / A.places;
-          r[q] = make_int4(v[0], v[1], v[2], v[3]);
-        }
-      }
-      const uint32_t bytes = L::A_BYTES + nb * (UP ? 4 : 32) * (MK * 2);
+      // B rows come in boxes of 32; rows past the block's last are not read
+      const int nb = (blk.z + 31) / 32;
+      const uint32_t bytes = L::A_BYTES + nb * 32 * (MK * 2);
       for (int kt = 0; kt < k_tiles; ++kt, ++kc) {
         const int s = kc % STAGES;
         if (kc >= STAGES) {
@@ -122,12 +104,7 @@ __global__ void __launch_bounds__(MTHREADS, 1) moe_tc_kernel(const __grid_consta
           else tma_load_3d(a_s, &tmA, full_bar(s), kt * MK, tile * 128, blk.x);
         }
         __syncwarp();  // the bytes are announced before any of them can arrive
-        if constexpr (UP) {
-          if (lane < nb) tma_gather4(b_s + lane * 512, &tmB, full_bar(s), kt * MK, r[0]);
-          if (lane + 32 < nb) tma_gather4(b_s + (lane + 32) * 512, &tmB, full_bar(s), kt * MK, r[1]);
-        } else {
-          if (lane < nb) tma_load_2d(b_s + lane * 32 * MK * 2, &tmB, full_bar(s), kt * MK, blk.y + lane * 32);
-        }
+        if (lane < nb) tma_load_2d(b_s + lane * 32 * MK * 2, &tmB, full_bar(s), kt * MK, blk.y + lane * 32);
         ++issued;
       }
     }
@@ -251,7 +228,7 @@ int moe_products_tc(const MoeArgs& A, int max_blocks, cudaStream_t s) {
   if (sms <= 0) sms = 148;
   using u64 = cuuint64_t;
   using u32 = cuuint32_t;
-  const u64 H = A.H, I = A.I, E = A.E, T = A.T, R = static_cast<u64>(A.T) * A.places;
+  const u64 H = A.H, I = A.I, E = A.E, R = static_cast<u64>(A.T) * A.places;
   CUtensorMap mgu, mx, md, mh;
   {
     const u64 dims[5] = {H, 8, 2, I / 8, E};
@@ -261,9 +238,9 @@ int moe_products_tc(const MoeArgs& A, int max_blocks, cudaStream_t s) {
     if ((rc = encode(&mgu, A.w_gu, 5, dims, strides, box)) != MMP_OK) return rc;
   }
   {
-    const u64 dims[2] = {H, T}, strides[1] = {static_cast<u64>(A.x_t) * 2};
-    const u32 box[2] = {MK, 1};
-    if ((rc = encode(&mx, A.x, 2, dims, strides, box)) != MMP_OK) return rc;
+    const u64 dims[2] = {H, R}, strides[1] = {H * 2};
+    const u32 box[2] = {MK, 32};
+    if ((rc = encode(&mx, A.xs, 2, dims, strides, box)) != MMP_OK) return rc;
   }
   {
     const u64 dr = static_cast<u64>(A.d_r) * 2, de = A.E > 1 ? static_cast<u64>(A.d_e) * 2 : H * dr;

@@ -811,7 +811,7 @@ def moe_experts(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, 
                   w_down.stride(0), w_down.stride(1), _p(weights), _rowmajor("weights", weights), _p(ids),
                   _rowmajor("ids", ids), _p(addend), _row(addend, "addend"), _p(out), _row(out, "out"), T, ids.shape[1],
                   H, I, E, _p(ws), ws.numel() * ws.element_size(), _p(error_word(x.device)), _stream(x),
-                  kernels=0 if T == 0 else 3 if T * ids.shape[1] <= MOE_FEW_PLACES else 6)
+                  kernels=0 if T == 0 else 3 if T * ids.shape[1] <= MOE_FEW_PLACES else 7)
     return out
 
 
@@ -835,5 +835,5 @@ def moe_layer(x: torch.Tensor, logits: torch.Tensor, w_gate_up: torch.Tensor, w_
                   w_gate_up.stride(1), _p(w_down), w_down.stride(0), w_down.stride(1), _p(addend), _row(addend, "addend"),
                   _p(out), _row(out, "out"), T, int(top_k), int(bool(renormalize)), int(bool(shared)), H, I, E, _p(ws),
                   ws.numel() * ws.element_size(), _p(error_word(x.device)), _stream(x),
-                  kernels=0 if T == 0 else 3 if T * places <= MOE_FEW_PLACES else 7)
+                  kernels=0 if T == 0 else 3 if T * places <= MOE_FEW_PLACES else 8)
     return out
