@@ -110,5 +110,7 @@ LAUNCHES = [0]  # kernel launches issued through this module (a counter for laun
 
 
 def call(name: str, *args, kernels: int = 1) -> None:
-    check(getattr(lib(), name)(*args), name)
+    rc = getattr(_lib or lib(), name)(*args)
+    if rc != MMP_OK:
+        check(rc, name)
     LAUNCHES[0] += kernels

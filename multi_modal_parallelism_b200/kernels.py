@@ -8,7 +8,7 @@ buffers, epilogue scales, workspaces) expose the fusions the layer uses.
 """
 from __future__ import annotations
 
-import contextlib
+import functools
 import math
 
 import torch
@@ -30,7 +30,7 @@ def _p(t: torch.Tensor | None):
 
 
 def _stream(t: torch.Tensor):
-    return torch.cuda.current_stream(t.device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def _cuda(name: str, *ts: torch.Tensor | None) -> None:
@@ -52,21 +52,30 @@ def _rowmajor(name: str, t: torch.Tensor) -> int:
     return t.stride(0)
 
 
-_NO_SWITCH = contextlib.nullcontext()
+def _device(name: str, *ts: torch.Tensor | None) -> int:
+    """The one CUDA device that all these tensors are on (its index). Wrappers of short kernels use it: at decode sizes the
+    time of a call on the host counts."""
+    d = ts[0].get_device()
+    for t in ts:
+        if t is not None and t.get_device() != d:
+            raise ValueError(f"{name}: tensors on several devices: {sorted({str(t.device) for t in ts if t is not None})}")
+    if d < 0:
+        _cuda(name, *ts)
+    return d
 
 
-def _on(t: torch.Tensor):
-    """The device of t as the current one (the library launches on the current device)."""
-    if not t.is_cuda or t.device.index == torch.cuda.current_device():
-        return _NO_SWITCH
-    return torch.cuda.device(t.device)
+def _call_on(d: int, name: str, *args, kernels: int = 1) -> None:
+    """_lib.call with device d as the current one (the library launches on the current device)."""
+    if d < 0 or d == torch._C._cuda_getDevice():
+        _lib.call(name, *args, kernels=kernels)
+    else:
+        with torch.cuda.device(d):
+            _lib.call(name, *args, kernels=kernels)
 
 
-def _one_device(name: str, *ts: torch.Tensor | None) -> None:
-    _cuda(name, *ts)
-    devs = {t.device for t in ts if t is not None}
-    if len(devs) > 1:
-        raise ValueError(f"{name}: tensors on several devices: {sorted(map(str, devs))}")
+def _err_and_stream(d: int, t: torch.Tensor):
+    w = _err_words.get(d)
+    return (error_word(t.device) if w is None else w).data_ptr(), _stream(t)
 
 
 def error_word(device: torch.device) -> torch.Tensor:
@@ -288,32 +297,29 @@ def qkv_mrope_kv_write(qkv: torch.Tensor, nq: int, nkv: int, head_dim: int, posi
     positions[axes[i], t] * inv_freq[i] (axes from rope_axes). Rows with slot_mapping < 0 are rotated into q_out and not
     cached. Angles are exact at any position."""
     name = "qkv_mrope_kv_write"
-    _one_device(name, qkv, positions, inv_freq, axes, q_out, key_cache, value_cache, slot_mapping)
-    for t in (qkv, q_out, key_cache, value_cache):
-        _dtype(name, t, BF16)
-    for t in (positions, slot_mapping):
-        _dtype(name, t, torch.int64)
-    _dtype(name, inv_freq, torch.float32)
-    _dtype(name, axes, torch.int32)
-    T = qkv.shape[0]
-    if qkv.dim() != 2 or qkv.shape[1] != (nq + 2 * nkv) * head_dim:
-        raise ValueError(f"{name}: qkv {tuple(qkv.shape)} is not [T, ({nq} + 2 * {nkv}) * {head_dim}]")
-    if positions.dim() != 2 or positions.shape[1] != T or (T > 1 and positions.stride(1) != 1):
-        raise ValueError(f"{name}: positions must be [axes, {T}] with contiguous rows, got {tuple(positions.shape)}")
-    if inv_freq.dim() != 1 or inv_freq.shape != axes.shape or not inv_freq.is_contiguous() or not axes.is_contiguous():
+    d = _device(name, qkv, positions, inv_freq, axes, q_out, key_cache, value_cache, slot_mapping)
+    if not qkv.dtype == q_out.dtype == key_cache.dtype == value_cache.dtype == BF16:
+        raise ValueError(f"{name}: qkv, q_out and the caches must be bf16")
+    if not positions.dtype == slot_mapping.dtype == torch.int64 or inv_freq.dtype != torch.float32 or axes.dtype != torch.int32:
+        raise ValueError(f"{name}: positions and slot_mapping must be int64, inv_freq fp32 and axes int32")
+    T, row = _rows(name, "qkv", qkv, (nq + 2 * nkv) * head_dim)
+    Tq, qo_b = _rows(name, "q_out", q_out, nq * head_dim)
+    ps = positions.shape
+    if len(ps) != 2 or ps[1] != T or Tq != T or (T > 1 and positions.stride(1) != 1):
+        raise ValueError(f"{name}: positions must be [axes, {T}] with contiguous rows, got {tuple(ps)}; q_out has {Tq} rows")
+    half = inv_freq.shape[0] if inv_freq.dim() == 1 else 0
+    if axes.shape != inv_freq.shape or not inv_freq.is_contiguous() or not axes.is_contiguous():
         raise ValueError(f"{name}: inv_freq and axes must be contiguous vectors of one length")
-    if slot_mapping.shape != (T,) or (T > 1 and slot_mapping.stride(0) != 1):
+    if slot_mapping.shape != (T,) or not slot_mapping.is_contiguous():
         raise ValueError(f"{name}: slot_mapping must be a contiguous [{T}]")
-    if q_out.shape != (T, nq * head_dim):
-        raise ValueError(f"{name}: q_out {tuple(q_out.shape)} is not [{T}, {nq * head_dim}]")
-    cb, ct, ch, blk, nb = _cache_strides(key_cache, value_cache)
-    if key_cache.shape != value_cache.shape or key_cache.shape[2:] != (nkv, head_dim):
-        raise ValueError(f"{name}: caches {tuple(key_cache.shape)} are not [blocks, block, {nkv}, {head_dim}]")
-    with _on(qkv):
-        _lib.call("mmp_mrope_kv_write", _p(qkv), _rowmajor("qkv", qkv), nq, nkv, head_dim, _p(positions),
-                  positions.stride(0), positions.shape[0], _p(inv_freq), _p(axes), 2 * inv_freq.shape[0], float(key_mult),
-                  _p(q_out), _rowmajor("q_out", q_out), _p(key_cache), _p(value_cache), cb, ct, ch, blk, nb,
-                  _p(slot_mapping), T, _p(error_word(qkv.device)), _stream(qkv))
+    cs, st = key_cache.shape, key_cache.stride()
+    if len(cs) != 4 or value_cache.shape != cs or value_cache.stride() != st or st[3] != 1 or cs[2] != nkv or cs[3] != head_dim:
+        raise ValueError(f"{name}: key/value caches must be [blocks, block, {nkv}, {head_dim}] views with equal strides, got "
+                         f"{tuple(cs)} and {tuple(value_cache.shape)}")
+    err, stream = _err_and_stream(d, qkv)
+    _call_on(d, "mmp_mrope_kv_write", qkv.data_ptr(), row, nq, nkv, head_dim, positions.data_ptr(), positions.stride(0), ps[0],
+             inv_freq.data_ptr(), axes.data_ptr(), 2 * half, key_mult, q_out.data_ptr(), qo_b, key_cache.data_ptr(),
+             value_cache.data_ptr(), st[0], st[1], st[2], cs[1], cs[0], slot_mapping.data_ptr(), T, err, stream)
     return q_out
 
 
@@ -722,10 +728,19 @@ def gdn_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, a: torch.Tens
 
 
 # ----------------------------------------------------------------------------- mixture of experts
-def _logits_dtype(name: str, logits: torch.Tensor) -> int:
-    if logits.dtype not in (torch.float32, BF16):
-        raise ValueError(f"{name}: logits must be fp32 or bf16, got {logits.dtype}")
-    return MMP_F32 if logits.dtype == torch.float32 else MMP_BF16
+MOE_FEW_PLACES = 1536  # tokens * places up to which the few-token kernels run
+_LOGITS = {torch.float32: MMP_F32, BF16: MMP_BF16}
+
+
+def _rows(name: str, what: str, t: torch.Tensor, cols: int) -> tuple[int, int]:
+    """(rows, row stride) of a [rows, cols] tensor with contiguous rows; a single row, which has no stride, counts as
+    aligned."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or shape[1] != cols or (stride[1] != 1 and cols > 1):
+        raise ValueError(f"{name}: {what} must be [rows, {cols}] with a contiguous last dimension, got {tuple(shape)} strides "
+                         f"{stride}")
+    n = shape[0]
+    return n, stride[0] if n > 1 else (cols + 7) // 8 * 8
 
 
 def moe_route(logits: torch.Tensor, top_k: int, weights: torch.Tensor | None = None, ids: torch.Tensor | None = None,
@@ -736,60 +751,65 @@ def moe_route(logits: torch.Tensor, top_k: int, weights: torch.Tensor | None = N
     shared: logits is [T, E + 1] and one more place follows, id E with weight sigmoid(logits[:, E]): an expert that every
     token takes, behind a gate of its own."""
     name = "moe_route"
-    _one_device(name, logits, weights, ids)
-    dt, l_t = _logits_dtype(name, logits), _rowmajor("logits", logits)
-    T, n, places = logits.shape[0], logits.shape[1] - bool(shared), int(top_k) + bool(shared)
+    d = _device(name, logits, weights, ids)
+    dt = _LOGITS.get(logits.dtype)
+    if dt is None or logits.dim() != 2:
+        raise ValueError(f"{name}: logits must be [T, experts] in fp32 or bf16, got {tuple(logits.shape)} {logits.dtype}")
+    sh = 1 if shared else 0
+    T, l_t = _rows(name, "logits", logits, logits.shape[1])
+    shape = (T, top_k + sh)
     if weights is None:
-        weights = torch.empty(T, places, dtype=torch.float32, device=logits.device)
+        weights = torch.empty(shape, dtype=torch.float32, device=logits.device)
+    elif weights.dtype != torch.float32 or weights.shape != shape or not weights.is_contiguous():
+        raise ValueError(f"{name}: weights must be a contiguous fp32 {shape}, got {tuple(weights.shape)} {weights.dtype}")
     if ids is None:
-        ids = torch.empty(T, places, dtype=torch.int32, device=logits.device)
-    _dtype(name, weights, torch.float32)
-    _dtype(name, ids, torch.int32)
-    for nm, t in (("weights", weights), ("ids", ids)):
-        if t.shape != (T, places) or not t.is_contiguous():
-            raise ValueError(f"{name}: {nm} must be a contiguous [{T}, {places}], got {tuple(t.shape)}")
-    with _on(logits):
-        _lib.call("mmp_moe_route", _p(logits), dt, l_t, T, n, int(top_k), int(bool(renormalize)), int(bool(shared)),
-                  _p(weights), _p(ids), _stream(logits))
+        ids = torch.empty(shape, dtype=torch.int32, device=logits.device)
+    elif ids.dtype != torch.int32 or ids.shape != shape or not ids.is_contiguous():
+        raise ValueError(f"{name}: ids must be a contiguous int32 {shape}, got {tuple(ids.shape)} {ids.dtype}")
+    _call_on(d, "mmp_moe_route", logits.data_ptr(), dt, l_t, T, logits.shape[1] - sh, top_k, 1 if renormalize else 0, sh,
+             weights.data_ptr(), ids.data_ptr(), _stream(logits))
     return weights, ids
 
 
+@functools.lru_cache(maxsize=256)
+def _moe_workspace_bytes(T: int, places: int, hidden: int, intermediate: int, experts: int) -> int:
+    return max(256, _lib.lib().mmp_moe_workspace_size(T, places, hidden, intermediate, experts))
+
+
 def moe_workspace(T: int, places: int, hidden: int, intermediate: int, experts: int, device: torch.device) -> torch.Tensor:
-    """Scratch for moe_experts / moe_layer of up to these sizes (places: ids per token, the shared expert's included).
-    Calls that may overlap on the GPU (two streams, two captured graphs) need one each."""
-    n = _lib.lib().mmp_moe_workspace_size(T, places, hidden, intermediate, experts)
-    return torch.empty(max(256, n), dtype=torch.uint8, device=device)
+    """Scratch for moe_experts / moe_layer of up to T tokens (places: ids per token, the shared expert's included). Calls that
+    may overlap on the GPU (two streams, two captured graphs) need one each."""
+    return torch.empty(_moe_workspace_bytes(T, places, hidden, intermediate, experts), dtype=torch.uint8, device=device)
 
 
-def _moe_common(name: str, x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, addend: torch.Tensor | None,
-                out: torch.Tensor | None, workspace: torch.Tensor | None, places: int):
-    for t in (x, w_gate_up, w_down, addend, out):
-        _dtype(name, t, BF16)
-    if x.dim() != 2 or w_gate_up.dim() != 3 or w_down.dim() != 3:
+def _moe_args(name: str, x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, addend: torch.Tensor | None,
+              out: torch.Tensor | None, workspace: torch.Tensor | None, places: int):
+    """Checks of what moe_experts and moe_layer share; the C arguments of the weights, of addend and out, and the rest."""
+    if not x.dtype == w_gate_up.dtype == w_down.dtype == BF16:
+        raise ValueError(f"{name}: x, w_gate_up and w_down must be bf16")
+    gs, ds = w_gate_up.shape, w_down.shape
+    if len(gs) != 3 or len(ds) != 3 or x.dim() != 2:
         raise ValueError(f"{name}: x [T, H], w_gate_up [E, 2 I, H] and w_down [E, H, I] expected")
-    T, H = x.shape
-    E, I = w_down.shape[0], w_down.shape[2]
-    if w_gate_up.shape != (E, 2 * I, H) or w_down.shape[1] != H:
-        raise ValueError(f"{name}: shapes disagree: x {tuple(x.shape)}, w_gate_up {tuple(w_gate_up.shape)}, "
-                         f"w_down {tuple(w_down.shape)}")
-    if w_gate_up.stride(2) != 1 or w_down.stride(2) != 1:
-        raise ValueError(f"{name}: the weights' last dimension must be contiguous")
+    E, H, I = ds
+    T, x_t = _rows(name, "x", x, H)
+    gu, dn = w_gate_up.stride(), w_down.stride()
+    if gs[0] != E or gs[1] != 2 * I or gs[2] != H or gu[2] != 1 or dn[2] != 1:
+        raise ValueError(f"{name}: w_gate_up {tuple(gs)} and w_down {tuple(ds)} must be [E, 2 I, H] and [E, H, I] with contiguous rows")
     if out is None:
-        out = torch.empty(T, H, dtype=BF16, device=x.device)
-    for nm, t in (("addend", addend), ("out", out)):
-        if t is not None and t.shape != (T, H):
-            raise ValueError(f"{name}: {nm} {tuple(t.shape)} is not [{T}, {H}]")
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    To, o_t = _rows(name, "out", out, H)
+    if To != T or out.dtype != BF16:
+        raise ValueError(f"{name}: out must be bf16 [{T}, {H}], got {tuple(out.shape)} {out.dtype}")
+    add, a_t = None, 0
+    if addend is not None:
+        Ta, a_t = _rows(name, "addend", addend, H)
+        if Ta != T or addend.dtype != BF16:
+            raise ValueError(f"{name}: addend must be bf16 [{T}, {H}], got {tuple(addend.shape)} {addend.dtype}")
+        add = addend.data_ptr()
     if workspace is None:
-        workspace = moe_workspace(T, places, H, I, E, x.device)
-    return T, H, I, E, out, workspace
-
-
-def _row(t: torch.Tensor | None, name: str) -> int:
-    """Row stride; of a single row, which has none, its length."""
-    if t is None:
-        return 0
-    s = _rowmajor(name, t)
-    return s if t.shape[0] > 1 else (t.shape[1] + 7) // 8 * 8
+        workspace = torch.empty(_moe_workspace_bytes(T, places, H, I, E), dtype=torch.uint8, device=x.device)
+    return (T, H, I, E, x_t, (w_gate_up.data_ptr(), gu[0], gu[1], w_down.data_ptr(), dn[0], dn[1]),
+            (add, a_t, out.data_ptr(), o_t), out, workspace, workspace.numel() * workspace.element_size())
 
 
 def moe_experts(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, weights: torch.Tensor, ids: torch.Tensor,
@@ -800,22 +820,20 @@ def moe_experts(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, 
     moe_route gives them). A place with id < 0 adds nothing; an id >= E is reported through the error word and adds nothing.
     out may be the addend. workspace: moe_workspace; without one, scratch is allocated for this call."""
     name = "moe_experts"
-    _one_device(name, x, w_gate_up, w_down, weights, ids, out, addend, workspace)
-    _dtype(name, weights, torch.float32)
-    _dtype(name, ids, torch.int32)
-    if ids.dim() != 2 or ids.shape[0] != x.shape[0] or weights.shape != ids.shape:
-        raise ValueError(f"{name}: weights and ids must be [{x.shape[0]}, places], got {tuple(weights.shape)} and {tuple(ids.shape)}")
-    T, H, I, E, out, ws = _moe_common(name, x, w_gate_up, w_down, addend, out, workspace, ids.shape[1])
-    with _on(x):
-        _lib.call("mmp_moe_experts", _p(x), _row(x, "x"), _p(w_gate_up), w_gate_up.stride(0), w_gate_up.stride(1), _p(w_down),
-                  w_down.stride(0), w_down.stride(1), _p(weights), _rowmajor("weights", weights), _p(ids),
-                  _rowmajor("ids", ids), _p(addend), _row(addend, "addend"), _p(out), _row(out, "out"), T, ids.shape[1],
-                  H, I, E, _p(ws), ws.numel() * ws.element_size(), _p(error_word(x.device)), _stream(x),
-                  kernels=0 if T == 0 else 3 if T * ids.shape[1] <= MOE_FEW_PLACES else 7)
+    d = _device(name, x, w_gate_up, w_down, weights, ids, out, addend, workspace)
+    if weights.dtype != torch.float32 or ids.dtype != torch.int32 or ids.dim() != 2 or ids.shape[0] != x.shape[0]:
+        raise ValueError(f"{name}: weights fp32 and ids int32 must be [{x.shape[0]}, places], got {tuple(weights.shape)} "
+                         f"{weights.dtype} and {tuple(ids.shape)} {ids.dtype}")
+    places = ids.shape[1]
+    _, id_t = _rows(name, "ids", ids, places)
+    Tw, w_t = _rows(name, "weights", weights, places)
+    if Tw != ids.shape[0]:
+        raise ValueError(f"{name}: weights {tuple(weights.shape)} and ids {tuple(ids.shape)} differ")
+    T, H, I, E, x_t, w, io, out, ws, n = _moe_args(name, x, w_gate_up, w_down, addend, out, workspace, places)
+    err, stream = _err_and_stream(d, x)
+    _call_on(d, "mmp_moe_experts", x.data_ptr(), x_t, *w, weights.data_ptr(), w_t, ids.data_ptr(), id_t, *io, T, places, H, I, E,
+             ws.data_ptr(), n, err, stream, kernels=0 if T == 0 else 3 if T * places <= MOE_FEW_PLACES else 7)
     return out
-
-
-MOE_FEW_PLACES = 1536  # tokens * places up to which the products stream weights without sorting through tensor memory
 
 
 def moe_layer(x: torch.Tensor, logits: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, top_k: int,
@@ -825,15 +843,17 @@ def moe_layer(x: torch.Tensor, logits: torch.Tensor, w_gate_up: torch.Tensor, w_
     [T, E] (shared: the same E columns, the last one the shared expert's gate; its weights are the last of w_gate_up and
     w_down)."""
     name = "moe_layer"
-    _one_device(name, x, logits, w_gate_up, w_down, out, addend, workspace)
-    dt, l_t, places = _logits_dtype(name, logits), _rowmajor("logits", logits), int(top_k) + bool(shared)
-    T, H, I, E, out, ws = _moe_common(name, x, w_gate_up, w_down, addend, out, workspace, places)
-    if logits.shape != (T, E):
+    d = _device(name, x, logits, w_gate_up, w_down, out, addend, workspace)
+    dt = _LOGITS.get(logits.dtype)
+    if dt is None:
+        raise ValueError(f"{name}: logits must be fp32 or bf16, got {logits.dtype}")
+    sh = 1 if shared else 0
+    places = top_k + sh
+    T, H, I, E, x_t, w, io, out, ws, n = _moe_args(name, x, w_gate_up, w_down, addend, out, workspace, places)
+    Tl, l_t = _rows(name, "logits", logits, E)
+    if Tl != T:
         raise ValueError(f"{name}: logits {tuple(logits.shape)} is not [{T}, {E}]")
-    with _on(x):
-        _lib.call("mmp_moe_layer", _p(x), _row(x, "x"), _p(logits), dt, l_t, _p(w_gate_up), w_gate_up.stride(0),
-                  w_gate_up.stride(1), _p(w_down), w_down.stride(0), w_down.stride(1), _p(addend), _row(addend, "addend"),
-                  _p(out), _row(out, "out"), T, int(top_k), int(bool(renormalize)), int(bool(shared)), H, I, E, _p(ws),
-                  ws.numel() * ws.element_size(), _p(error_word(x.device)), _stream(x),
-                  kernels=0 if T == 0 else 3 if T * places <= MOE_FEW_PLACES else 8)
+    err, stream = _err_and_stream(d, x)
+    _call_on(d, "mmp_moe_layer", x.data_ptr(), x_t, logits.data_ptr(), dt, l_t, *w, *io, T, top_k, 1 if renormalize else 0, sh, H, I,
+             E, ws.data_ptr(), n, err, stream, kernels=0 if T == 0 else 3 if T * places <= MOE_FEW_PLACES else 8)
     return out
