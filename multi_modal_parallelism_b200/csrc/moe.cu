@@ -24,14 +24,18 @@ struct RouteParams {
 };
 
 // Floats as unsigned integers of the same order; 0 stands for "not to be chosen" (-inf, NaN, already taken): every
-// other float maps above it.
+// other float maps above it. +inf is the largest float: in fp32 the two tie; no bf16 is equal to it, there only the value
+// is clamped.
+constexpr float LARGEST = 3.402823466e38f;
+template <bool F32>
 __device__ __forceinline__ uint32_t order_key(float v) {
   if (!(v > -INFINITY)) return 0u;
-  const uint32_t u = __float_as_uint(fminf(v, 3.402823466e38f) + 0.f);  // + 0: the two zeros are one value
+  if (F32) v = fminf(v, LARGEST);
+  const uint32_t u = __float_as_uint(v + 0.f);  // + 0: the two zeros are one value
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
-  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+  return fminf(__uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k), LARGEST);
 }
 
 template <bool F32>
@@ -40,7 +44,8 @@ __device__ __forceinline__ float load_logit(const void* p, int64_t i) {
   else return bf2f(static_cast<const bf16*>(p)[i]);
 }
 
-// One token by one warp; lane j ends with place j's expert and weight (j < top_k + shared). V values a lane.
+// One token by one warp; lane j ends with place j's expert and weight (j < top_k + shared). V values a lane. A bf16 key has
+// 16 bits: with the index below it one maximum finds the largest key and, among equals, the lowest index.
 template <int V, bool F32>
 __device__ __forceinline__ void route_token(const RouteParams& P, int t, int lane, int& id, float& w) {
   const int64_t row = static_cast<int64_t>(t) * P.l_t;
@@ -48,50 +53,62 @@ __device__ __forceinline__ void route_token(const RouteParams& P, int t, int lan
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     const int e = lane + 32 * j;
-    key[j] = e < P.E ? order_key(load_logit<F32>(P.logits, row + e)) : 0u;
+    key[j] = e < P.E ? order_key<F32>(load_logit<F32>(P.logits, row + e)) : 0u;
   }
   float gate = 0.f;
-  if (P.shared && lane == 0) gate = load_logit<F32>(P.logits, row + P.E);
-  uint32_t best = 0;
+  if (P.shared) gate = load_logit<F32>(P.logits, row + P.E);
+  auto largest = [&]() {
+    uint32_t m = key[0];
 #pragma unroll
-  for (int j = 0; j < V; ++j) best = max(best, key[j]);
-  const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-  const float vmax = key_value(top);
+    for (int j = 1; j < V; ++j) m = max(m, key[j]);
+    return __reduce_max_sync(0xffffffffu, m);
+  };
   float z = 0.f;
+  const uint32_t top = largest();
+  const float vmax = key_value(top);
   if (!P.renorm) {
 #pragma unroll
     for (int j = 0; j < V; ++j) z += key[j] ? expf(key_value(key[j]) - vmax) : 0.f;
     z = warp_sum(z);
   }
   id = -1;
-  w = 0.f;
-  uint32_t m = top;
-  for (int k = 0; k < P.top_k && m; ++k) {  // m == 0: nothing left to choose
-    // lowest index that holds the largest key
-    int at = 1 << 30;
+  uint32_t mine = 0;
+  if constexpr (F32) {
+    uint32_t m = top;
+    for (int k = 0; k < P.top_k && m; ++k) {  // m == 0: nothing left to choose
+      int at = 1 << 30;
 #pragma unroll
-    for (int j = V - 1; j >= 0; --j) at = key[j] == m ? lane + 32 * j : at;
-    at = __reduce_min_sync(0xffffffffu, at);
-    if (lane == k) {
-      id = at;
-      w = expf(key_value(m) - vmax);
-    }
-    best = 0;
+      for (int j = V - 1; j >= 0; --j) at = key[j] == m ? lane + 32 * j : at;
+      at = __reduce_min_sync(0xffffffffu, at);
+      if (lane == k) {
+        id = at;
+        mine = m;
+      }
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      if (lane + 32 * j == at) key[j] = 0u;
-      best = max(best, key[j]);
+      for (int j = 0; j < V; ++j) key[j] = lane + 32 * j == at ? 0u : key[j];
+      m = largest();
     }
-    m = __reduce_max_sync(0xffffffffu, best);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) key[j] = key[j] ? (key[j] & 0xffff0000u) | (0xffffu - (lane + 32 * j)) : 0u;
+    for (int k = 0; k < P.top_k; ++k) {
+      const uint32_t m = largest();
+      if (m == 0) break;
+      if (lane == k) {
+        id = 0xffff - static_cast<int>(m & 0xffffu);
+        // the low half of a bf16's key: 0, or all ones below zero
+        mine = (m & 0xffff0000u) | ((m & 0x80000000u) ? 0u : 0xffffu);
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) key[j] = key[j] == m ? 0u : key[j];
+    }
   }
+  w = id >= 0 ? expf(key_value(mine) - vmax) : 0.f;
   if (P.renorm) z = warp_sum(w);
   if (id >= 0) w /= z;
-  if (P.shared) {
-    const float g = __shfl_sync(0xffffffffu, gate, 0);
-    if (lane == P.top_k) {
-      id = P.E;
-      w = 1.f / (1.f + expf(-g));
-    }
+  if (P.shared && lane == P.top_k) {
+    id = P.E;
+    w = 1.f / (1.f + expf(-gate));
   }
 }
 
@@ -182,6 +199,7 @@ __global__ void __launch_bounds__(1024) moe_plan_few(const RouteAndPlan Q) {
   __shared__ int cnt[MOE_MAX_EXPERTS];
   __shared__ int2 warp_tot[32];
   __shared__ short s_e[MOE_FEW_PLACES], s_rank[MOE_FEW_PLACES];
+  pdl_trigger();  // the next kernel may start; it waits for this one's end before it reads the plan
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int R = A.T * A.places;
   for (int e = tid; e < A.E; e += 1024) cnt[e] = 0;
@@ -288,7 +306,9 @@ __device__ __forceinline__ uint4 ld_weight(const bf16* p) {
 }
 __device__ __forceinline__ uint4 ld_rows(const bf16* p) { return __ldcg(reinterpret_cast<const uint4*>(p)); }
 
-constexpr int SLAB = 8;  // 32-wide k chunks whose weights a warp holds in registers at once (2 rows x 8 x 16 bytes a lane)
+// 32-wide k chunks whose weights a warp holds in registers at once (2 rows x 4 x 16 bytes a lane). With 8 (two blocks of the
+// up kernel an SM instead of three) 64 tokens x 8 of 256 experts (H 2048, I 512) took 265 us, with 4 they take 239.
+constexpr int SLAB = 4;
 
 // acc[f] (16 rows x 8 tokens) += W[16 rows, k] X[8 tokens, k]^T over the warp's k chunks c0, c0 + step, ... < c1. ra / rb:
 // this lane's two weight rows (null: a row outside the matrix), xr[f]: this lane's token row of group f (null: none).
@@ -360,7 +380,7 @@ __device__ __forceinline__ void up_pass(const MoeArgs& A, const int4 rec, int ba
 }
 
 // Block (i, r): columns 8 i .. 8 i + 7 of h for the rows of the r-th live expert.
-__global__ void __launch_bounds__(UP_WARPS * 32, 2) moe_up_few(const MoeArgs A) {
+__global__ void __launch_bounds__(UP_WARPS * 32, 3) moe_up_few(const MoeArgs A) {
   __shared__ float4 red[UP_WARPS * 4 * 32];
   pdl_wait();
   pdl_trigger();  // after the wait: what the plan wrote is then visible to the next kernel before its own wait
@@ -514,6 +534,7 @@ __global__ void __launch_bounds__(256) moe_combine(const MoeArgs A) {
 template <template <int, bool> class F, typename... Args>
 int by_width(int E, bool f32, Args&&... args) {
   if (E <= 64) return f32 ? F<2, true>::go(args...) : F<2, false>::go(args...);
+  if (E <= 160) return f32 ? F<5, true>::go(args...) : F<5, false>::go(args...);
   if (E <= 256) return f32 ? F<8, true>::go(args...) : F<8, false>::go(args...);
   return f32 ? F<32, true>::go(args...) : F<32, false>::go(args...);
 }
