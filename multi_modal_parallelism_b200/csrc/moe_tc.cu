@@ -10,8 +10,10 @@
 //     took four times as long: one such instruction every 66 clocks).
 //   * down: A is 128 rows of Wd, B the expert's consecutive rows of h. fp32 results per place go to y, and moe_combine sums
 //     each token's places in their order.
-// One persistent block an SM; warp 0 streams both operands through a ring of shared-memory stages across tiles, one lane of
-// warp 1 issues the MMAs into one of two TMEM accumulators, warps 2-5 drain the other.
+// One persistent block an SM, two of them a pair on 256 weight rows (cta_group::2): each loads its own weights and half of the
+// rows, so a stage of the MMAs takes 32 KB an SM instead of 48. Warp 0 streams both operands through a ring of shared-memory
+// stages across tiles, one lane of the leader's warp 1 issues the MMAs into one of two TMEM accumulators, warps 2-5 drain the
+// other.
 #include <algorithm>
 
 #include "moe.cuh"
@@ -24,8 +26,8 @@ constexpr int MK = 64, MTHREADS = 192;
 
 template <int STAGES>
 struct MLayout {
-  static constexpr int A_BYTES = 128 * MK * 2;
-  static constexpr int B_BYTES = MOE_BLOCK_ROWS * MK * 2;
+  static constexpr int A_BYTES = 128 * MK * 2;                  // this block's 128 weight rows
+  static constexpr int B_BYTES = MOE_BLOCK_ROWS / 2 * MK * 2;   // its half of the rows
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int BARS = STAGES * STAGE_BYTES;  // full[S], empty[S], acc_full[2], acc_empty[2]
   static constexpr int TMEM_SLOT = BARS + 8 * (2 * STAGES + 4);
@@ -33,19 +35,50 @@ struct MLayout {
   static constexpr int DYN = ABORT + 4 + 1024;
 };
 
-__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int u, int v) {
+// TMA loads into this block's shared memory that complete on a barrier of either block of the pair (no multicast).
+__device__ __forceinline__ void pair_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
   asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];\n"
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];\n"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void pair_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5}], [%2];\n"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void pair_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int u, int v) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5, %6, %7}], "
+      "[%2];\n"
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(u), "r"(v) : "memory");
 }
+__device__ __forceinline__ void pair_mma(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+      ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate));
+}
+// arrives on the barrier at this offset in both blocks once the MMAs issued so far have completed
+__device__ __forceinline__ void pair_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"
+               ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
+}
+__device__ __forceinline__ void pair_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+
+// Two blocks of a cluster are a pair on one 256-row tile: each loads its 128 weight rows and half of the block's rows of B,
+// the leader (rank 0) issues the MMAs for both (cta_group::2), each drains its own 128 rows of the accumulator.
 template <bool UP, int STAGES>
-__global__ void __launch_bounds__(MTHREADS, 1) moe_tc_kernel(const __grid_constant__ CUtensorMap tmA,
-                                                             const __grid_constant__ CUtensorMap tmB, const MoeArgs A, int tiles) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
+    moe_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const MoeArgs A, int tiles) {
   using L = MLayout<STAGES>;
   extern __shared__ uint8_t dsmem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_addr(smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint32_t rank;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(rank));
+  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
   const int k_tiles = ((UP ? A.H : A.I) + MK - 1) / MK;
   auto full_bar = [&](int s) { return sbase + L::BARS + 8 * s; };
   auto empty_bar = [&](int s) { return sbase + L::BARS + 8 * (STAGES + s); };
@@ -56,12 +89,12 @@ __global__ void __launch_bounds__(MTHREADS, 1) moe_tc_kernel(const __grid_consta
 
   if (tid == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(full_bar(s), 1);
-      mbar_init(empty_bar(s), 1);
+      mbar_init(full_bar(s), 1);   // the leader's announcement of both blocks' bytes (used in the leader alone)
+      mbar_init(empty_bar(s), 1);  // the leader's commit
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(accf_bar(b), 1);
-      mbar_init(acce_bar(b), 4);  // one elected lane per epilogue warp
+      mbar_init(acce_bar(b), 8);  // one lane of each epilogue warp of both blocks (used in the leader alone)
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -69,11 +102,11 @@ __global__ void __launch_bounds__(MTHREADS, 1) moe_tc_kernel(const __grid_consta
     asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(&tmB)) : "memory");
   }
   if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(tmem_slot)), "r"(512));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(tmem_slot)), "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::);
   }
   tc_fence_before();
-  __syncthreads();
+  pair_sync();  // both blocks' barriers are set up and their TMEM is allocated
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
@@ -84,12 +117,13 @@ __global__ void __launch_bounds__(MTHREADS, 1) moe_tc_kernel(const __grid_consta
   if (warp == 0) {
     int kc = 0;
     bool ok = true;
-    for (int it = blockIdx.x; it < nitems && ok; it += gridDim.x) {
+    for (int it = pair; it < nitems && ok; it += npairs) {
       const int4 blk = __ldcg(A.blocks + it / tiles);
-      const int tile = it % tiles;
-      // B rows come in boxes of 32; rows past the block's last are not read
-      const int nb = (blk.z + 31) / 32;
-      const uint32_t bytes = L::A_BYTES + nb * 32 * (MK * 2);
+      const int tile = (it % tiles) * 2 + rank;
+      // this block's half of the MMA's N rows, in boxes of 32 (what lies past them is not read)
+      const int half = (blk.z + 15) / 16 * 8;
+      const int nb = (half + 31) / 32;
+      const uint32_t bytes = 2 * (L::A_BYTES + nb * 32 * (MK * 2));
       for (int kt = 0; kt < k_tiles; ++kt, ++kc) {
         const int s = kc % STAGES;
         if (kc >= STAGES) {
@@ -98,23 +132,23 @@ __global__ void __launch_bounds__(MTHREADS, 1) moe_tc_kernel(const __grid_consta
           if (!ok) break;
         }
         const uint32_t a_s = sbase + s * L::STAGE_BYTES, b_s = a_s + L::A_BYTES;
+        const uint32_t bar = mapa(full_bar(s), 0);  // the leader's; bytes may arrive there before they are announced
         if (lane == 0) {
-          mbar_expect_tx(full_bar(s), bytes);
-          if (UP) tma_load_5d(a_s, &tmA, full_bar(s), kt * MK, 0, 0, tile * 8, blk.x);
-          else tma_load_3d(a_s, &tmA, full_bar(s), kt * MK, tile * 128, blk.x);
+          if (rank == 0) mbar_expect_tx(full_bar(s), bytes);
+          if (UP) pair_load_5d(a_s, &tmA, bar, kt * MK, 0, 0, tile * 8, blk.x);
+          else pair_load_3d(a_s, &tmA, bar, kt * MK, tile * 128, blk.x);
         }
-        __syncwarp();  // the bytes are announced before any of them can arrive
-        if (lane < nb) tma_load_2d(b_s + lane * 32 * MK * 2, &tmB, full_bar(s), kt * MK, blk.y + lane * 32);
+        if (lane < nb) pair_load_2d(b_s + lane * 32 * MK * 2, &tmB, bar, kt * MK, blk.y + static_cast<int>(rank) * half + lane * 32);
         ++issued;
       }
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       int kc = 0, tc = 0;
-      for (int it = blockIdx.x; it < nitems && !*abort_flag; it += gridDim.x, ++tc) {
+      for (int it = pair; it < nitems && !*abort_flag; it += npairs, ++tc) {
         const int4 blk = __ldcg(A.blocks + it / tiles);
-        const uint32_t idesc = umma_idesc_mn(128, (blk.z + 15) / 16 * 16);
+        const uint32_t idesc = umma_idesc_mn(256, (blk.z + 15) / 16 * 16);
         const int buf = tc & 1;
         if (tc >= 2 && !mbar_wait(acce_bar(buf), ((tc >> 1) - 1) & 1, abort_flag, A.err)) break;
         tc_fence_after();
@@ -126,20 +160,20 @@ __global__ void __launch_bounds__(MTHREADS, 1) moe_tc_kernel(const __grid_consta
           const uint32_t a_s = sbase + s * L::STAGE_BYTES, b_s = a_s + L::A_BYTES;
 #pragma unroll
           for (int kk = 0; kk < MK / 16; ++kk)
-            umma_f16(tmem + buf * 256, umma_desc(a_s + kk * 32), umma_desc(b_s + kk * 32), idesc, kt != 0 || kk != 0);
-          umma_commit(empty_bar(s));
+            pair_mma(tmem + buf * 256, umma_desc(a_s + kk * 32), umma_desc(b_s + kk * 32), idesc, kt != 0 || kk != 0);
+          pair_commit(empty_bar(s));
         }
         if (!ok) break;
-        umma_commit(accf_bar(buf));
+        pair_commit(accf_bar(buf));
       }
     }
     __syncwarp();
   } else {
     const int q = warp & 3;  // TMEM lanes 32 q .. 32 q + 31
     int tc = 0;
-    for (int it = blockIdx.x; it < nitems; it += gridDim.x, ++tc) {
+    for (int it = pair; it < nitems; it += npairs, ++tc) {
       const int4 blk = __ldcg(A.blocks + it / tiles);
-      const int tile = it % tiles;
+      const int tile = (it % tiles) * 2 + rank;
       const int buf = tc & 1;
       bool ok = mbar_wait(accf_bar(buf), (tc >> 1) & 1, abort_flag, A.err);
       ok = __all_sync(0xffffffffu, ok && !*abort_flag);
@@ -162,7 +196,7 @@ __global__ void __launch_bounds__(MTHREADS, 1) moe_tc_kernel(const __grid_consta
             const float gt = up ? got : mine0, uu = up ? mine1 : got;
             const int c = cb + j + up;
             // h is rounded to bf16, the type of the second product's operands
-            if (c < blk.z && i < A.I) A.h[static_cast<int64_t>(blk.y + c) * A.I + i] = f2bf(gt / (1.f + __expf(-gt)) * uu);
+            if (c < blk.z && i < A.I) A.h[static_cast<int64_t>(blk.y + c) * A.I + i] = f2bf(silu(gt) * uu);
           }
         } else {
           const int col = tile * 128 + q * 32 + lane;
@@ -174,19 +208,29 @@ __global__ void __launch_bounds__(MTHREADS, 1) moe_tc_kernel(const __grid_consta
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(acce_bar(buf)) : "memory");
+      if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(mapa(acce_bar(buf), 0)) : "memory");
     }
   }
 
+  // teardown: after an abort the copies of either block may still be in flight; the leader's barriers show both blocks', the
+  // other block lets the microseconds pass that they take
   if (tid == 0 && *abort_flag) {
-    for (int i = max(0, issued - STAGES); i < issued; ++i) mbar_drain(full_bar(i % STAGES), (i / STAGES) & 1);
+    if (rank == 0) {
+      for (int i = max(0, issued - STAGES); i < issued; ++i) mbar_drain(full_bar(i % STAGES), (i / STAGES) & 1);
+    } else {
+      const long long t0 = clock64();
+      while (clock64() - t0 < WAIT_BUDGET_CYCLES / 16) {
+      }
+    }
   }
   tc_fence_before();
   __syncthreads();
+  pair_sync();  // no block leaves while the other may still signal its barriers or read its operands
   if (warp == 0) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512));
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512));
   }
+  pair_sync();
 }
 
 int encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
@@ -200,7 +244,7 @@ int encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims,
 
 template <bool UP>
 int launch_products(const CUtensorMap& ma, const CUtensorMap& mb, const MoeArgs& A, int tiles, int max_blocks, int sms, cudaStream_t s) {
-  constexpr int STAGES = 4;
+  constexpr int STAGES = 6;
   using L = MLayout<STAGES>;
   auto kern = moe_tc_kernel<UP, STAGES>;
   static bool set[64] = {};
@@ -211,7 +255,7 @@ int launch_products(const CUtensorMap& ma, const CUtensorMap& mb, const MoeArgs&
     if (e != cudaSuccess) return mmp_set_error(MMP_ERR_CUDA, "mmp_moe_experts: shared memory attribute: %s", cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) set[dev] = true;
   }
-  const int grid = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(max_blocks) * tiles, sms));
+  const int grid = 2 * static_cast<int>(std::min<int64_t>(static_cast<int64_t>(max_blocks) * tiles, std::max(1, sms / 2)));
   cudaError_t e = launch_kind(1, kern, dim3(grid), dim3(MTHREADS), L::DYN, s, nullptr, 0, ma, mb, A, tiles);
   if (e != cudaSuccess) return mmp_set_error(MMP_ERR_CUDA, "mmp_moe_experts: %s", cudaGetErrorString(e));
   return MMP_OK;
@@ -253,8 +297,8 @@ int moe_products_tc(const MoeArgs& A, int max_blocks, cudaStream_t s) {
     const u32 box[2] = {MK, 32};
     if ((rc = encode(&mh, A.h, 2, dims, strides, box)) != MMP_OK) return rc;
   }
-  if ((rc = launch_products<true>(mgu, mx, A, (A.I + 63) / 64, max_blocks, sms, s)) != MMP_OK) return rc;
-  if ((rc = launch_products<false>(md, mh, A, (A.H + 127) / 128, max_blocks, sms, s)) != MMP_OK) return rc;
+  if ((rc = launch_products<true>(mgu, mx, A, (A.I + 127) / 128, max_blocks, sms, s)) != MMP_OK) return rc;
+  if ((rc = launch_products<false>(md, mh, A, (A.H + 255) / 256, max_blocks, sms, s)) != MMP_OK) return rc;
   return mmp_check_launch("mmp_moe_experts");
 }
 
