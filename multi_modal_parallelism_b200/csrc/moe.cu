@@ -10,8 +10,11 @@
 //   down: a block takes 16 columns of the output for ALL experts, its warps take (expert, k range) tasks and leave 16 fp32
 //         a place in shared memory, then sum each token's places in their order: no atomics, no partial results in HBM.
 #include <algorithm>
+#include <cooperative_groups.h>
 
 #include "moe.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace mmp {
 namespace {
@@ -169,22 +172,20 @@ __device__ __forceinline__ int place_expert(const MoeArgs& A, int p, bool report
 }
 
 // From an expert's row count (thread i has expert E - 1 - i: the last expert, which every token may share, comes first)
-// to its records and row blocks. Returns the expert's first sorted row.
-__device__ __forceinline__ int plan_expert(const MoeArgs& A, int e, int n, int2* warp_tot) {
+// to its record and, with `blocks`, its row blocks, written by the block that has `write`. Returns its first sorted row.
+__device__ __forceinline__ int plan_expert(const MoeArgs& A, int e, int n, int2* warp_tot, bool blocks, bool write) {
   int2 total;
-  int2 pre = scan_block(make_int2(n, n > 0 ? 1 : 0), warp_tot, total);
-  const int off = pre.x;
-  if (n > 0) A.recs[pre.y] = make_int4(e, off, n, 0);
-  if (threadIdx.x == 0) A.header->nact = total.y;
-  __syncthreads();
   const int nb = (n + MOE_BLOCK_ROWS - 1) / MOE_BLOCK_ROWS;
-  pre = scan_block(make_int2(0, nb), warp_tot, total);
-  if (threadIdx.x == 0) A.header->nblk = total.y;
-  for (int b = 0; b < nb; ++b) {  // blocks of nearly equal size
-    const int r0 = static_cast<int>(static_cast<int64_t>(n) * b / nb), r1 = static_cast<int>(static_cast<int64_t>(n) * (b + 1) / nb);
-    A.blocks[pre.y + b] = make_int4(e, off + r0, r1 - r0, 0);
+  const int2 pre = scan_block(make_int2(n, blocks ? nb : n > 0 ? 1 : 0), warp_tot, total);
+  if (!write) return pre.x;
+  if (blocks) {
+    for (int b = 0; b < nb; ++b) A.blocks[pre.y + b] = make_int4(e, pre.x, n, b);
+    if (threadIdx.x == 0) A.header->nblk = total.y;
+  } else {
+    if (n > 0) A.recs[pre.y] = make_int4(e, pre.x, n, 0);
+    if (threadIdx.x == 0) A.header->nact = total.y;
   }
-  return off;
+  return pre.x;
 }
 
 struct RouteAndPlan {
@@ -224,7 +225,7 @@ __global__ void __launch_bounds__(1024) moe_plan_few(const RouteAndPlan Q) {
   }
   __syncthreads();
   const int e = A.E - 1 - tid;
-  const int off = plan_expert(A, e, e >= 0 ? cnt[e] : 0, warp_tot);
+  const int off = plan_expert(A, e, e >= 0 ? cnt[e] : 0, warp_tot, false, true);
   __syncthreads();
   if (e >= 0) cnt[e] = off;
   __syncthreads();
@@ -236,51 +237,51 @@ __global__ void __launch_bounds__(1024) moe_plan_few(const RouteAndPlan Q) {
   }
 }
 
-// Many places: counts of each chunk, one block for the scan over chunks and experts, then the scatter.
-__global__ void __launch_bounds__(256) moe_count(const MoeArgs A) {
-  __shared__ int cnt[MOE_MAX_EXPERTS];
-  for (int e = threadIdx.x; e < A.E; e += 256) cnt[e] = 0;
+// The plan of many places by one cluster: every block counts its share of the places in shared memory, reads the others'
+// counts there (distributed shared memory), scans the experts for itself and scatters its share. One launch: counting,
+// scanning and scattering as three took 16 us of 434 for 4096 tokens x 8 places.
+constexpr int PLAN_BLOCKS = 8;
+
+__global__ void __cluster_dims__(PLAN_BLOCKS, 1, 1) __launch_bounds__(1024) moe_plan_many(const MoeArgs A) {
+  __shared__ int cnt[MOE_MAX_EXPERTS], at[MOE_MAX_EXPERTS];
+  __shared__ int2 warp_tot[32];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int me = static_cast<int>(cluster.block_rank()), tid = threadIdx.x;
+  pdl_wait();
+  pdl_trigger();
+  const int64_t R = static_cast<int64_t>(A.T) * A.places;
+  const int p0 = static_cast<int>(R * me / PLAN_BLOCKS), p1 = static_cast<int>(R * (me + 1) / PLAN_BLOCKS);
+  for (int e = tid; e < A.E; e += 1024) cnt[e] = 0;
   __syncthreads();
-  const int R = A.T * A.places, p0 = blockIdx.x * MOE_CHUNK, p1 = min(R, p0 + MOE_CHUNK);
-  for (int p = p0 + threadIdx.x; p < p1; p += 256) {
+  for (int p = p0 + tid; p < p1; p += 1024) {
     const int e = place_expert(A, p, true);
     if (e >= 0) atomicAdd(&cnt[e], 1);
   }
-  __syncthreads();
-  for (int e = threadIdx.x; e < A.E; e += 256) A.counts[static_cast<int64_t>(blockIdx.x) * A.E + e] = cnt[e];
-}
-
-__global__ void __launch_bounds__(1024) moe_scan(const MoeArgs A, int chunks) {
-  __shared__ int2 warp_tot[32];
-  const int e = A.E - 1 - static_cast<int>(threadIdx.x);
-  int n = 0;
+  cluster.sync();
+  const int e = A.E - 1 - tid;
+  int n = 0, before = 0;
   if (e >= 0)
-    for (int c = 0; c < chunks; ++c) n += A.counts[static_cast<int64_t>(c) * A.E + e];
-  int at = plan_expert(A, e, n, warp_tot);
-  if (e >= 0)
-    for (int c = 0; c < chunks; ++c) {  // counts become the chunk's first sorted row of the expert
-      int* q = A.counts + static_cast<int64_t>(c) * A.E + e;
-      const int k = *q;
-      *q = at;
-      at += k;
+#pragma unroll
+    for (int b = 0; b < PLAN_BLOCKS; ++b) {
+      const int c = cluster.map_shared_rank(cnt, b)[e];
+      n += c;
+      before += b < me ? c : 0;
     }
-}
-
-__global__ void __launch_bounds__(256) moe_scatter(const MoeArgs A) {
-  __shared__ int at[MOE_MAX_EXPERTS];
-  for (int e = threadIdx.x; e < A.E; e += 256) at[e] = A.counts[static_cast<int64_t>(blockIdx.x) * A.E + e];
-  __syncthreads();
-  const int R = A.T * A.places, p0 = blockIdx.x * MOE_CHUNK, p1 = min(R, p0 + MOE_CHUNK);
-  for (int p = p0 + threadIdx.x; p < p1; p += 256) {
-    const int e = place_expert(A, p, false);
-    const int r = e >= 0 ? atomicAdd(&at[e], 1) : -1;
-    if (e >= 0) A.rows[r] = p;
+  const int off = plan_expert(A, e, n, warp_tot, true, me == 0);
+  if (e >= 0) at[e] = off + before;
+  cluster.sync();  // no block leaves while its counts are read
+  for (int p = p0 + tid; p < p1; p += 1024) {
+    const int q = place_expert(A, p, false);
+    const int r = q >= 0 ? atomicAdd(&at[q], 1) : -1;
+    if (q >= 0) A.rows[r] = p;
     A.pos[p] = r;
   }
 }
 
 // Each token's row to the sorted rows of its places: block (token), read once, written once a place.
 __global__ void __launch_bounds__(256) moe_sort_rows(const MoeArgs A) {
+  pdl_wait();
+  pdl_trigger();
   const int64_t t = blockIdx.x;
   for (int c = threadIdx.x * 8; c < A.H; c += 256 * 8) {
     const uint4 v = ld16(A.x + t * A.x_t + c);
@@ -583,13 +584,12 @@ int few_products(const MoeArgs& A, cudaStream_t s) {
 }
 
 int many_products(const MoeArgs& A, const MoeLayout& L, cudaStream_t s) {
-  moe_count<<<L.chunks, 256, 0, s>>>(A);
-  moe_scan<<<1, 1024, 0, s>>>(A, L.chunks);
-  moe_scatter<<<L.chunks, 256, 0, s>>>(A);
-  moe_sort_rows<<<A.T, 256, 0, s>>>(A);
-  int rc = mmp_check_launch("mmp_moe_experts");
+  cudaError_t e = launch_kind(1, moe_plan_many, dim3(PLAN_BLOCKS), dim3(1024), 0, s, nullptr, 0, A);
+  if (e != cudaSuccess) return mmp_set_error(MMP_ERR_CUDA, "mmp_moe_experts: %s", cudaGetErrorString(e));
+  e = launch_kind(1, moe_sort_rows, dim3(A.T), dim3(256), 0, s, nullptr, 0, A);
+  if (e != cudaSuccess) return mmp_set_error(MMP_ERR_CUDA, "mmp_moe_experts: %s", cudaGetErrorString(e));
+  const int rc = moe_products_tc(A, L.max_blocks, s);
   if (rc != MMP_OK) return rc;
-  if ((rc = moe_products_tc(A, L.max_blocks, s)) != MMP_OK) return rc;
   moe_combine<<<A.T, 256, 0, s>>>(A);
   return mmp_check_launch("mmp_moe_experts");
 }
@@ -633,7 +633,6 @@ void place_workspace(MoeArgs& A, const MoeLayout& L, void* workspace) {
   A.blocks = reinterpret_cast<int4*>(w + L.blocks);
   A.rows = reinterpret_cast<int*>(w + L.rows);
   A.pos = reinterpret_cast<int*>(w + L.pos);
-  A.counts = reinterpret_cast<int*>(w + L.counts);
   A.xs = reinterpret_cast<bf16*>(w + L.xs);
   A.h = reinterpret_cast<bf16*>(w + L.h);
   A.y = reinterpret_cast<float*>(w + L.y);

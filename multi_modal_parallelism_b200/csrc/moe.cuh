@@ -12,7 +12,6 @@ namespace mmp {
 constexpr int MOE_MAX_EXPERTS = 1024;  // experts in the weight tensors (one thread each in the scan)
 constexpr int MOE_MAX_TOPK = 32;       // one lane each in the router
 constexpr int MOE_FEW_PLACES = 1536;   // the few-token kernels keep 16 fp32 a place in shared memory (96 KB)
-constexpr int MOE_CHUNK = 2048;        // places a counting block takes
 constexpr int MOE_BLOCK_ROWS = 256;    // sorted rows of one expert that the tensor-core kernels take at a time (MMA N)
 
 struct MoeHeader {
@@ -23,8 +22,8 @@ struct MoeHeader {
 
 // Workspace offsets in bytes, every part 256-byte aligned.
 struct MoeLayout {
-  size_t header, recs, blocks, rows, pos, weights, ids, counts, xs, h, y, bytes;
-  int chunks, max_blocks;
+  size_t header, recs, blocks, rows, pos, weights, ids, xs, h, y, bytes;
+  int max_blocks;
 };
 
 inline size_t moe_align(size_t n) { return (n + 255) / 256 * 256; }
@@ -33,7 +32,6 @@ inline MoeLayout moe_layout(int64_t T, int places, int H, int I, int E) {
   MoeLayout L;
   const size_t R = static_cast<size_t>(T) * places;
   const bool few = R <= MOE_FEW_PLACES;
-  L.chunks = static_cast<int>((R + MOE_CHUNK - 1) / MOE_CHUNK);
   L.max_blocks = static_cast<int>(R / MOE_BLOCK_ROWS) + E;  // sum over experts of ceil(n / block) is at most this
   size_t at = 0;
   auto part = [&](size_t n) { const size_t o = at; at += moe_align(n); return o; };
@@ -44,7 +42,6 @@ inline MoeLayout moe_layout(int64_t T, int places, int H, int I, int E) {
   L.pos = part(R * 4);
   L.weights = part(R * 4);
   L.ids = part(R * 4);
-  L.counts = part(static_cast<size_t>(L.chunks) * E * 4);
   L.xs = part(few ? 0 : R * H * 2);
   L.h = part(R * I * 2);
   L.y = part(few ? 0 : R * H * 4);
@@ -64,10 +61,9 @@ struct MoeArgs {
   int T, places, H, I, E;
   MoeHeader* header;
   int4* recs;     // {expert, first sorted row, rows, 0} of the experts with rows, by falling expert
-  int4* blocks;   // {expert, first sorted row, rows, 0} of the row blocks
+  int4* blocks;   // {expert, its first sorted row, its rows, index among its blocks} of the row blocks
   int* rows;      // sorted row -> place
   int* pos;       // place -> sorted row, -1 where the place has no expert
-  int* counts;    // [chunk][expert]
   bf16* xs;       // [sorted row][H]: x in the order of the rows (tensor-core path)
   bf16* h;        // [sorted row][I]
   float* y;       // [sorted row][H]

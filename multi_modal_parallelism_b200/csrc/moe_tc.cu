@@ -6,8 +6,9 @@
 // about 250 rows an expert the layer is bound by reading the weights, above it by the MMAs.
 //   * up: the A tile is 64 gate and 64 up rows, alternating in groups of 8: one box of a 5-D tensor map over the
 //     [expert][gate | up][row] layout. Gate and up values of one column of h then sit 8 lanes apart in one warp. B are the
-//     expert's rows of xs, x sorted by a kernel before this one (gathered by TMA, four rows an instruction, the same kernel
-//     took four times as long: one such instruction every 66 clocks).
+//     expert's rows of xs, x sorted by a kernel before this one: 25 us for 4096 tokens x 8 places, where gathering from x
+//     inside this kernel cost 100 (16-byte copies by a warp for each stage: the fence that hands them to the MMA waits for
+//     all of a warp's copies) and 550 us (TMA gathers of four rows, one every 66 clocks).
 //   * down: A is 128 rows of Wd, B the expert's consecutive rows of h. fp32 results per place go to y, and moe_combine sums
 //     each token's places in their order.
 // One persistent block an SM, two of them a pair on 256 weight rows (cta_group::2): each loads its own weights and half of the
@@ -66,6 +67,23 @@ __device__ __forceinline__ void pair_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
 
+__device__ __forceinline__ void arrive_leader(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(mapa(bar, 0)) : "memory");
+}
+
+// Work item `it`: a row block of an expert and a 256-row weight tile. The items of one tile over an expert's blocks follow
+// one another, so that its weights come from HBM once (2 of 8 large experts, four blocks each: block by block their 117 MB
+// would pass through L2 four times).
+struct Item { int expert, row0, n, tile; };
+__device__ __forceinline__ Item moe_item(const MoeArgs& A, int it, int tiles) {
+  const int b = it / tiles;
+  const int4 r = __ldcg(A.blocks + b);
+  const int nb = (r.z + MOE_BLOCK_ROWS - 1) / MOE_BLOCK_ROWS, q = it - (b - r.w) * tiles, tile = q / nb, j = q - tile * nb;
+  // blocks of nearly equal size
+  const int r0 = static_cast<int>(static_cast<int64_t>(r.z) * j / nb), r1 = static_cast<int>(static_cast<int64_t>(r.z) * (j + 1) / nb);
+  return {r.x, r.y + r0, r1 - r0, tile};
+}
+
 // Two blocks of a cluster are a pair on one 256-row tile: each loads its 128 weight rows and half of the block's rows of B,
 // the leader (rank 0) issues the MMAs for both (cta_group::2), each drains its own 128 rows of the accumulator.
 template <bool UP, int STAGES>
@@ -118,10 +136,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
     int kc = 0;
     bool ok = true;
     for (int it = pair; it < nitems && ok; it += npairs) {
-      const int4 blk = __ldcg(A.blocks + it / tiles);
-      const int tile = (it % tiles) * 2 + rank;
+      const Item blk = moe_item(A, it, tiles);
+      const int tile = blk.tile * 2 + rank;
       // this block's half of the MMA's N rows, in boxes of 32 (what lies past them is not read)
-      const int half = (blk.z + 15) / 16 * 8;
+      const int half = (blk.n + 15) / 16 * 8;
       const int nb = (half + 31) / 32;
       const uint32_t bytes = 2 * (L::A_BYTES + nb * 32 * (MK * 2));
       for (int kt = 0; kt < k_tiles; ++kt, ++kc) {
@@ -135,10 +153,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
         const uint32_t bar = mapa(full_bar(s), 0);  // the leader's; bytes may arrive there before they are announced
         if (lane == 0) {
           if (rank == 0) mbar_expect_tx(full_bar(s), bytes);
-          if (UP) pair_load_5d(a_s, &tmA, bar, kt * MK, 0, 0, tile * 8, blk.x);
-          else pair_load_3d(a_s, &tmA, bar, kt * MK, tile * 128, blk.x);
+          if (UP) pair_load_5d(a_s, &tmA, bar, kt * MK, 0, 0, tile * 8, blk.expert);
+          else pair_load_3d(a_s, &tmA, bar, kt * MK, tile * 128, blk.expert);
         }
-        if (lane < nb) pair_load_2d(b_s + lane * 32 * MK * 2, &tmB, bar, kt * MK, blk.y + static_cast<int>(rank) * half + lane * 32);
+        if (lane < nb) pair_load_2d(b_s + lane * 32 * MK * 2, &tmB, bar, kt * MK, blk.row0 + static_cast<int>(rank) * half + lane * 32);
         ++issued;
       }
     }
@@ -147,8 +165,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
     if (lane == 0 && rank == 0) {
       int kc = 0, tc = 0;
       for (int it = pair; it < nitems && !*abort_flag; it += npairs, ++tc) {
-        const int4 blk = __ldcg(A.blocks + it / tiles);
-        const uint32_t idesc = umma_idesc_mn(256, (blk.z + 15) / 16 * 16);
+        const uint32_t idesc = umma_idesc_mn(256, (moe_item(A, it, tiles).n + 15) / 16 * 16);
         const int buf = tc & 1;
         if (tc >= 2 && !mbar_wait(acce_bar(buf), ((tc >> 1) - 1) & 1, abort_flag, A.err)) break;
         tc_fence_after();
@@ -172,8 +189,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
     const int q = warp & 3;  // TMEM lanes 32 q .. 32 q + 31
     int tc = 0;
     for (int it = pair; it < nitems; it += npairs, ++tc) {
-      const int4 blk = __ldcg(A.blocks + it / tiles);
-      const int tile = (it % tiles) * 2 + rank;
+      const Item blk = moe_item(A, it, tiles);
+      const int tile = blk.tile * 2 + rank;
       const int buf = tc & 1;
       bool ok = mbar_wait(accf_bar(buf), (tc >> 1) & 1, abort_flag, A.err);
       ok = __all_sync(0xffffffffu, ok && !*abort_flag);
@@ -181,7 +198,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
       tc_fence_after();
       const uint32_t t_lane = tmem + (static_cast<uint32_t>(q * 32) << 16) + buf * 256;
 #pragma unroll 1
-      for (int cb = 0; cb < blk.z; cb += 16) {
+      for (int cb = 0; cb < blk.n; cb += 16) {
         uint32_t v[16];
         tmem_ld16_nw(t_lane + cb, v);
         tmem_wait();
@@ -196,19 +213,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
             const float gt = up ? got : mine0, uu = up ? mine1 : got;
             const int c = cb + j + up;
             // h is rounded to bf16, the type of the second product's operands
-            if (c < blk.z && i < A.I) A.h[static_cast<int64_t>(blk.y + c) * A.I + i] = f2bf(silu(gt) * uu);
+            if (c < blk.n && i < A.I) A.h[static_cast<int64_t>(blk.row0 + c) * A.I + i] = f2bf(silu(gt) * uu);
           }
         } else {
           const int col = tile * 128 + q * 32 + lane;
-          float* y = A.y + static_cast<int64_t>(blk.y + cb) * A.H + col;
+          float* y = A.y + static_cast<int64_t>(blk.row0 + cb) * A.H + col;
 #pragma unroll
           for (int j = 0; j < 16; ++j)
-            if (cb + j < blk.z && col < A.H) y[static_cast<int64_t>(j) * A.H] = __uint_as_float(v[j]);
+            if (cb + j < blk.n && col < A.H) y[static_cast<int64_t>(j) * A.H] = __uint_as_float(v[j]);
         }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(mapa(acce_bar(buf), 0)) : "memory");
+      if (lane == 0) arrive_leader(acce_bar(buf));
     }
   }
 

@@ -832,7 +832,7 @@ def moe_experts(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, 
     T, H, I, E, x_t, w, io, out, ws, n = _moe_args(name, x, w_gate_up, w_down, addend, out, workspace, places)
     err, stream = _err_and_stream(d, x)
     _call_on(d, "mmp_moe_experts", x.data_ptr(), x_t, *w, weights.data_ptr(), w_t, ids.data_ptr(), id_t, *io, T, places, H, I, E,
-             ws.data_ptr(), n, err, stream, kernels=0 if T == 0 else 3 if T * places <= MOE_FEW_PLACES else 7)
+             ws.data_ptr(), n, err, stream, kernels=0 if T == 0 else 3 if T * places <= MOE_FEW_PLACES else 5)
     return out
 
 
@@ -855,5 +855,5 @@ def moe_layer(x: torch.Tensor, logits: torch.Tensor, w_gate_up: torch.Tensor, w_
         raise ValueError(f"{name}: logits {tuple(logits.shape)} is not [{T}, {E}]")
     err, stream = _err_and_stream(d, x)
     _call_on(d, "mmp_moe_layer", x.data_ptr(), x_t, logits.data_ptr(), dt, l_t, *w, *io, T, top_k, 1 if renormalize else 0, sh, H, I,
-             E, ws.data_ptr(), n, err, stream, kernels=0 if T == 0 else 3 if T * places <= MOE_FEW_PLACES else 8)
+             E, ws.data_ptr(), n, err, stream, kernels=0 if T == 0 else 3 if T * places <= MOE_FEW_PLACES else 5)
     return out
