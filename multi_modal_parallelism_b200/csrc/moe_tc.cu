@@ -138,10 +138,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
     for (int it = pair; it < nitems && ok; it += npairs) {
       const Item blk = moe_item(A, it, tiles);
       const int tile = blk.tile * 2 + rank;
-      // this block's half of the MMA's N rows, in boxes of 32 (what lies past them is not read)
+      // this block's half of the MMA's N rows, in boxes of 64 (what lies past it is not read; boxes of 32 or 16
+      // copy less and cost 6 and 20 % more where the MMAs bound the kernel: each box is an instruction)
       const int half = (blk.n + 15) / 16 * 8;
-      const int nb = (half + 31) / 32;
-      const uint32_t bytes = 2 * (L::A_BYTES + nb * 32 * (MK * 2));
+      const int nb = (half + 63) / 64;
+      const uint32_t bytes = 2 * (L::A_BYTES + nb * 64 * (MK * 2));
       for (int kt = 0; kt < k_tiles; ++kt, ++kc) {
         const int s = kc % STAGES;
         if (kc >= STAGES) {
@@ -156,7 +157,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
           if (UP) pair_load_5d(a_s, &tmA, bar, kt * MK, 0, 0, tile * 8, blk.expert);
           else pair_load_3d(a_s, &tmA, bar, kt * MK, tile * 128, blk.expert);
         }
-        if (lane < nb) pair_load_2d(b_s + lane * 32 * MK * 2, &tmB, bar, kt * MK, blk.row0 + static_cast<int>(rank) * half + lane * 32);
+        if (lane < nb) pair_load_2d(b_s + lane * 64 * MK * 2, &tmB, bar, kt * MK, blk.row0 + static_cast<int>(rank) * half + lane * 64);
         ++issued;
       }
     }
@@ -300,7 +301,7 @@ int moe_products_tc(const MoeArgs& A, int max_blocks, cudaStream_t s) {
   }
   {
     const u64 dims[2] = {H, R}, strides[1] = {H * 2};
-    const u32 box[2] = {MK, 32};
+    const u32 box[2] = {MK, 64};
     if ((rc = encode(&mx, A.xs, 2, dims, strides, box)) != MMP_OK) return rc;
   }
   {
@@ -311,7 +312,7 @@ int moe_products_tc(const MoeArgs& A, int max_blocks, cudaStream_t s) {
   }
   {
     const u64 dims[2] = {I, R}, strides[1] = {I * 2};
-    const u32 box[2] = {MK, 32};
+    const u32 box[2] = {MK, 64};
     if ((rc = encode(&mh, A.h, 2, dims, strides, box)) != MMP_OK) return rc;
   }
   if ((rc = launch_products<true>(mgu, mx, A, (A.I + 127) / 128, max_blocks, sms, s)) != MMP_OK) return rc;
