@@ -392,8 +392,8 @@ int mmp_gdn_prefill_tc(const void* q, int64_t q_t, int64_t q_h, const void* k, i
  * mmp_moe_workspace_size(T, places, H, I, E) bytes, scratch of this call alone: calls that may overlap on the GPU, captured
  * ones among them, need one each.
  *
- * mmp_moe_layer: both from the logits ([T, E], columns as mmp_moe_route takes them); with few tokens routing and the sort by expert are one
- * launch. E counts the experts of the weight tensors, the shared one (their last) included. */
+ * mmp_moe_layer: both from the logits ([T, E], columns as mmp_moe_route takes them); with at most 8 tokens (and
+ * 64 places) routing, both products and the sum are one cooperative launch. E counts the experts of the weight tensors, the shared one (their last) included. */
 int mmp_moe_route(const void* logits, int logits_dtype, int64_t l_t, int T, int E, int top_k, int renormalize, int shared,
                   float* weights, int32_t* ids, void* stream);
 size_t mmp_moe_workspace_size(int T, int places, int H, int I, int E);

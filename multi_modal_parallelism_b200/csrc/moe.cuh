@@ -5,6 +5,8 @@
 // rows [off, off + n), sorted row r belongs to place rows[r]. The order of places inside an expert is whatever the
 // counting gave: every row is computed by itself, so no result depends on it.
 #pragma once
+#include <algorithm>
+
 #include "mmp_common.cuh"
 
 namespace mmp {
@@ -12,17 +14,26 @@ namespace mmp {
 constexpr int MOE_MAX_EXPERTS = 1024;  // experts in the weight tensors (one thread each in the scan)
 constexpr int MOE_MAX_TOPK = 32;       // one lane each in the router
 constexpr int MOE_FEW_PLACES = 1536;   // the few-token kernels keep 16 fp32 a place in shared memory (96 KB)
+constexpr int MOE_TINY_TOKENS = 8, MOE_TINY_PLACES = 64;  // up to which every block of the few-token kernels plans for itself
 constexpr int MOE_BLOCK_ROWS = 256;    // sorted rows of one expert that the tensor-core kernels take at a time (MMA N)
 
 struct MoeHeader {
-  int nact;  // experts with rows
-  int nblk;  // row blocks of the tensor-core kernels
+  int ngroups;  // groups of the few-token kernels
+  int nblk;     // row blocks of the tensor-core kernels
   int pad[2];
 };
 
+// Few-token kernels: at most 16 places that one expert serves together.
+struct MoeGroup {
+  int e, n, pad[2];
+  int place[16];
+};
+
+inline bool moe_is_few(int64_t T, int places, int E) { return T * places <= MOE_FEW_PLACES; }
+
 // Workspace offsets in bytes, every part 256-byte aligned.
 struct MoeLayout {
-  size_t header, recs, blocks, rows, pos, weights, ids, xs, h, y, bytes;
+  size_t header, groups, blocks, rows, pos, weights, ids, xs, h, y, bytes;
   int max_blocks;
 };
 
@@ -30,16 +41,17 @@ inline size_t moe_align(size_t n) { return (n + 255) / 256 * 256; }
 
 inline MoeLayout moe_layout(int64_t T, int places, int H, int I, int E) {
   MoeLayout L;
-  const size_t R = static_cast<size_t>(T) * places;
-  const bool few = R <= MOE_FEW_PLACES;
-  L.max_blocks = static_cast<int>(R / MOE_BLOCK_ROWS) + E;  // sum over experts of ceil(n / block) is at most this
+  const int64_t R = T * places;
+  const bool few = moe_is_few(T, places, E);
+  // the sum over experts of ceil(n / b) is at most R / b + E, and R
+  L.max_blocks = static_cast<int>(std::min<int64_t>(R, R / MOE_BLOCK_ROWS + E));
   size_t at = 0;
   auto part = [&](size_t n) { const size_t o = at; at += moe_align(n); return o; };
   L.header = part(sizeof(MoeHeader));
-  L.recs = part(static_cast<size_t>(E) * 16);
-  L.blocks = part(static_cast<size_t>(L.max_blocks) * 16);
-  L.rows = part(R * 4);
-  L.pos = part(R * 4);
+  L.groups = part(few ? std::min<size_t>(R, R / 8 + E) * sizeof(MoeGroup) : 0);
+  L.blocks = part(few ? 0 : static_cast<size_t>(L.max_blocks) * 16);
+  L.rows = part(few ? 0 : R * 4);
+  L.pos = part(few ? 0 : R * 4);
   L.weights = part(R * 4);
   L.ids = part(R * 4);
   L.xs = part(few ? 0 : R * H * 2);
@@ -60,15 +72,32 @@ struct MoeArgs {
   bf16* out; int64_t o_t;
   int T, places, H, I, E;
   MoeHeader* header;
-  int4* recs;     // {expert, first sorted row, rows, 0} of the experts with rows, by falling expert
+  MoeGroup* groups;
   int4* blocks;   // {expert, its first sorted row, its rows, index among its blocks} of the row blocks
   int* rows;      // sorted row -> place
   int* pos;       // place -> sorted row, -1 where the place has no expert
   bf16* xs;       // [sorted row][H]: x in the order of the rows (tensor-core path)
-  bf16* h;        // [sorted row][I]
+  bf16* h;        // [sorted row][I]; few-token kernels: [place][I]
   float* y;       // [sorted row][H]
   int* err;
 };
+
+struct RouteParams {
+  const void* logits; int64_t l_t;
+  int T, E, top_k, renorm, shared;
+  float* weights; int32_t* ids;  // [T, top_k + shared], contiguous
+};
+
+// How the few-token kernels take a call: tiny (every block plans for itself, and routes where there are logits), rows of a
+// group.
+struct MoeFewPlan { bool tiny; int rows; };
+inline MoeFewPlan moe_few_plan(const MoeArgs& A) {
+  const int R = A.T * A.places;
+  const bool tiny = A.T <= MOE_TINY_TOKENS && R <= MOE_TINY_PLACES;
+  return {tiny, tiny || R <= 4 * A.E ? 8 : 16};
+}
+// The few-token products (moe_few.cu) and the sum into A.out.
+int moe_products_few(const MoeArgs& A, const RouteParams& P, bool f32, const MoeFewPlan& plan, cudaStream_t s);
 
 // The tensor-core path (moe_tc.cu): gate/up and down products of a planned call into A.h and A.y.
 int moe_products_tc(const MoeArgs& A, int max_blocks, cudaStream_t s);

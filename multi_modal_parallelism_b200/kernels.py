@@ -728,7 +728,18 @@ def gdn_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, a: torch.Tens
 
 
 # ----------------------------------------------------------------------------- mixture of experts
-MOE_FEW_PLACES = 1536  # tokens * places up to which the few-token kernels run
+def _moe_launches(T: int, places: int, route: bool) -> int:
+    """Kernels of one call (the library's rules on sizes)."""
+    n = T * places
+    if n == 0:
+        return 0
+    if T <= 8 and n <= 64:
+        return 1  # one cooperative launch
+    if n <= 1536:
+        return 3 + (route and T > 32)  # plan (with the routing of up to 32 tokens), up, down
+    return 5 + route  # plan, sorted rows, up, down, sum
+
+
 _LOGITS = {torch.float32: MMP_F32, BF16: MMP_BF16}
 
 
@@ -832,14 +843,14 @@ def moe_experts(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, 
     T, H, I, E, x_t, w, io, out, ws, n = _moe_args(name, x, w_gate_up, w_down, addend, out, workspace, places)
     err, stream = _err_and_stream(d, x)
     _call_on(d, "mmp_moe_experts", x.data_ptr(), x_t, *w, weights.data_ptr(), w_t, ids.data_ptr(), id_t, *io, T, places, H, I, E,
-             ws.data_ptr(), n, err, stream, kernels=0 if T == 0 else 3 if T * places <= MOE_FEW_PLACES else 5)
+             ws.data_ptr(), n, err, stream, kernels=_moe_launches(T, places, False))
     return out
 
 
 def moe_layer(x: torch.Tensor, logits: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, top_k: int,
               out: torch.Tensor | None = None, renormalize: bool = True, shared: bool = False,
               addend: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
-    """moe_route and moe_experts in one call: with few tokens, routing, sorting and both products are three launches. logits
+    """moe_route and moe_experts in one call: up to 8 tokens it is one launch, up to 32 three. logits
     [T, E] (shared: the same E columns, the last one the shared expert's gate; its weights are the last of w_gate_up and
     w_down)."""
     name = "moe_layer"
@@ -855,5 +866,5 @@ def moe_layer(x: torch.Tensor, logits: torch.Tensor, w_gate_up: torch.Tensor, w_
         raise ValueError(f"{name}: logits {tuple(logits.shape)} is not [{T}, {E}]")
     err, stream = _err_and_stream(d, x)
     _call_on(d, "mmp_moe_layer", x.data_ptr(), x_t, logits.data_ptr(), dt, l_t, *w, *io, T, top_k, 1 if renormalize else 0, sh, H, I,
-             E, ws.data_ptr(), n, err, stream, kernels=0 if T == 0 else 3 if T * places <= MOE_FEW_PLACES else 5)
+             E, ws.data_ptr(), n, err, stream, kernels=_moe_launches(T, places, True))
     return out
