@@ -47,28 +47,35 @@ __device__ __forceinline__ uint4 lds16(uint32_t a) {
 
 constexpr int STEP = 64;
 
-// A warp's queue of D steps for NF groups of 8 tokens. In a slot: 2 x 2 x 512 bytes of weights (half step, row half), then
-// 2 x NF x 512 bytes of token rows, 16 bytes a lane each.
-template <int NF, int D>
+// A warp's queue of D steps for MT tiles of 16 weight rows and NF groups of 8 tokens. In a slot: 2 x MT x 2 x 512 bytes of
+// weights (half step, tile, 8 rows), then 2 x NF x 512 bytes of token rows, 16 bytes a lane each. Weights pass through shared
+// memory once in, once out; with 16 tokens their rows did as much again, so that two tiles share them there.
+template <int MT, int NF, int D>
 struct Queue {
-  static constexpr int SLOT = (4 + 2 * NF) * 512;
+  static constexpr int SLOT = (4 * MT + 2 * NF) * 512;
   static constexpr int BYTES = D * SLOT;
   uint32_t base;  // this lane's 16 bytes of slot 0
   int put = 0, get = 0;
 
-  // rows ra and rb from column k on (zeros past K; of rb, where !second)
-  __device__ __forceinline__ void weights(int slot, const bf16* ra, const bf16* rb, bool second, int k, int K) const {
+  // this lane's row of every 8: row + tile * of_tile + (second 8) * of_half, from column k on (zeros past K, and in the 8-row
+  // pieces from `pieces` on)
+  __device__ __forceinline__ void weights(int slot, const bf16* row, int64_t of_tile, int64_t of_half, int pieces, int k, int K) const {
     const uint32_t s = base + slot * SLOT;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const bool in = k + h * 32 < K;
-      const int kk = in ? k + h * 32 : 0;
-      copy_weight(s + h * 1024, ra + kk, in);
-      copy_weight(s + h * 1024 + 512, rb + kk, in && second);
+      const bf16* p = row + (in ? k + h * 32 : 0);
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const bool have = m * 2 + j < pieces;
+          copy_weight(s + ((h * MT + m) * 2 + j) * 512, have ? p + m * of_tile + j * of_half : p, in && have);
+        }
     }
   }
   __device__ __forceinline__ void rows(int slot, const bf16* const (&xr)[NF], const bool (&have)[NF], int k, int K) const {
-    const uint32_t s = base + slot * SLOT + 2048;
+    const uint32_t s = base + slot * SLOT + 2048 * MT;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const bool in = k + h * 32 < K;
@@ -81,23 +88,38 @@ struct Queue {
     copy_commit();
     put = put + 1 == D ? 0 : put + 1;
   }
-  // acc[f] (16 rows x 8 tokens) += the oldest step
-  __device__ __forceinline__ void pop(float (&acc)[NF][4]) {
+  // acc[m][f] (16 rows x 8 tokens) += the oldest step
+  __device__ __forceinline__ void pop(float (&acc)[MT][NF][4]) {
     copy_wait<D - 1>();
     const uint32_t s = base + get * SLOT;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint4 a = lds16(s + h * 1024), b = lds16(s + h * 1024 + 512);
+      uint4 x[NF];
 #pragma unroll
-      for (int f = 0; f < NF; ++f) {
-        const uint4 x = lds16(s + 2048 + (h * NF + f) * 512);
-        mma_16816(acc[f], a.x, b.x, a.y, b.y, x.x, x.y);
-        mma_16816(acc[f], a.z, b.z, a.w, b.w, x.z, x.w);
+      for (int f = 0; f < NF; ++f) x[f] = lds16(s + 2048 * MT + (h * NF + f) * 512);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const uint4 a = lds16(s + (h * MT + m) * 1024), b = lds16(s + (h * MT + m) * 1024 + 512);
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+          mma_16816(acc[m][f], a.x, b.x, a.y, b.y, x[f].x, x[f].y);
+          mma_16816(acc[m][f], a.z, b.z, a.w, b.w, x[f].z, x[f].w);
+        }
       }
     }
     get = get + 1 == D ? 0 : get + 1;
   }
 };
+
+template <int MT, int NF>
+__device__ __forceinline__ void clear(float (&acc)[MT][NF][4]) {
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[m][f][c] = 0.f;
+}
 
 // ------------------------------------------------------------------------------------------------ plan of a few places
 struct TinyGroup {
@@ -209,24 +231,25 @@ struct Group {
 // ------------------------------------------------------------------------------------------------ up
 constexpr int UP_WARPS = 8;
 
-// Units u = u0, u0 + stride, ... by a crew of 8 warps: columns 8 (u % units) .. of h for group u / units. red: 8 * NF * 32
-// float4 of the crew; sync(): its barrier.
-template <int NF, int D, typename G, typename Sync>
+// Units u = u0, u0 + stride, ... by a crew of 8 warps: columns 8 MT (u % units) .. of h for group u / units. red:
+// 8 * MT * NF * 32 float4 of the crew; sync(): its barrier.
+template <int MT, int NF, int D, typename G, typename Sync>
 __device__ __forceinline__ void up_units(const MoeArgs& A, const G* groups, int ngroups, int u0, int stride, int warp, int lane,
-                                         Queue<NF, D>& q, float4* red, Sync sync) {
+                                         Queue<MT, NF, D>& q, float4* red, Sync sync) {
   const int g4 = lane >> 2, t4 = lane & 3;
-  const int units = A.I / 8, total = ngroups * units, steps = (A.H + STEP - 1) / STEP;
+  const int units = (A.I + 8 * MT - 1) / (8 * MT), total = ngroups * units, steps = (A.H + STEP - 1) / STEP;
   const int mine = steps > warp ? (steps - warp + UP_WARPS - 1) / UP_WARPS : 0;  // steps warp, warp + 8, ... of a unit
 
   // the unit whose steps are being requested, and the group of the one after it
-  int pu = u0, ps = 0;
-  const bf16 *ra = nullptr, *rb = nullptr, *xr[NF];
+  int pu = u0, ps = 0, pieces = 0;
+  const bf16 *row = nullptr, *xr[NF];
   bool have[NF];
   Group<NF> next;
   if (pu < total) next.load(groups + pu / units, g4);
   auto open = [&]() {
-    ra = A.w_gu + next.e * A.gu_e + static_cast<int64_t>(pu % units * 8 + g4) * A.gu_r + t4 * 8;
-    rb = ra + A.I * A.gu_r;
+    const int i0 = pu % units * 8 * MT;
+    row = A.w_gu + next.e * A.gu_e + static_cast<int64_t>(i0 + g4) * A.gu_r + t4 * 8;
+    pieces = min(MT, (A.I - i0) / 8) * 2;
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
       xr[f] = A.x + next.place[f] / A.places * A.x_t + t4 * 8;
@@ -238,7 +261,7 @@ __device__ __forceinline__ void up_units(const MoeArgs& A, const G* groups, int 
   auto request = [&]() {
     if (pu < total && mine > 0) {
       const int k = (warp + ps * UP_WARPS) * STEP, kl = A.H - t4 * 8;  // this lane's columns start 8 t4 in
-      q.weights(q.put, ra, rb, true, k, kl);
+      q.weights(q.put, row, 8 * A.gu_r, A.I * A.gu_r, pieces, k, kl);
       q.rows(q.put, xr, have, k, kl);
       if (++ps == mine) {
         ps = 0;
@@ -253,34 +276,37 @@ __device__ __forceinline__ void up_units(const MoeArgs& A, const G* groups, int 
 
   int round = 0;
   for (int u = u0; u < total; u += stride, ++round) {
-    float acc[NF][4];
-#pragma unroll
-    for (int f = 0; f < NF; ++f)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) acc[f][c] = 0.f;
+    float acc[MT][NF][4];
+    clear(acc);
     for (int s = 0; s < mine; ++s) {
       q.pop(acc);
       request();
     }
 #pragma unroll
-    for (int f = 0; f < NF; ++f) red[(warp * NF + f) * 32 + lane] = make_float4(acc[f][0], acc[f][1], acc[f][2], acc[f][3]);
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        const float* c = acc[m][f];
+        red[(warp * MT * NF + m * NF + f) * 32 + lane] = make_float4(c[0], c[1], c[2], c[3]);
+      }
     sync();
-    const int f = (warp - round) & (UP_WARPS - 1);
-    if (f < NF) {  // one warp for each 8 tokens, another one each round
-      float4 v = red[f * 32 + lane];
+    const int b = (warp - round) & (UP_WARPS - 1);
+    if (b < MT * NF) {  // one warp for each 8 columns and 8 tokens, another one each round
+      const int m = b / NF, f = b % NF;
+      float4 v = red[b * 32 + lane];
 #pragma unroll
       for (int w = 1; w < UP_WARPS; ++w) {
-        const float4 o = red[(w * NF + f) * 32 + lane];
+        const float4 o = red[(w * MT * NF + b) * 32 + lane];
         v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
       }
       const auto* gr = groups + u / units;
-      const int n = plan_load(gr, &gr->n), i = u % units * 8 + g4;
+      const int n = plan_load(gr, &gr->n), i = (u % units * MT + m) * 8 + g4;
       // h is rounded to bf16, the type of the second product's operands: half a step of 2^-8 relative, as the output's own
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int row = f * 8 + t4 * 2 + c;
+        const int r = f * 8 + t4 * 2 + c;
         const float gt = c ? v.y : v.x, up = c ? v.w : v.z;
-        if (row < n) A.h[static_cast<int64_t>(plan_load(gr, &gr->place[row])) * A.I + i] = f2bf(silu(gt) * up);
+        if (r < n && i < A.I) A.h[static_cast<int64_t>(plan_load(gr, &gr->place[r])) * A.I + i] = f2bf(silu(gt) * up);
       }
     }
     sync();
@@ -299,22 +325,21 @@ __device__ __forceinline__ int down_splits(int ngroups, int steps, int warps, in
   return static_cast<int>(__reduce_min_sync(0xffffffffu, len << 8 | sp) & 255u);
 }
 
-// Output columns r0 .. r0 + 15: the warps' tasks (group, k range) into val [split][place][16]. ready() is called by every warp
+// Output columns r0 .. r0 + 16 MT - 1: the warps' tasks (group, k range) into val [split][place][16 MT]. ready() is called by every warp
 // once its first weights are requested, and returns when h is written.
-template <int NF, int D, typename G, typename Ready>
+template <int MT, int NF, int D, typename G, typename Ready>
 __device__ __forceinline__ void down_tasks(const MoeArgs& A, const G* groups, int ngroups, int splits, int r0, int warp, int warps,
-                                           int lane, Queue<NF, D>& q, float* val, Ready ready) {
+                                           int lane, Queue<MT, NF, D>& q, float* val, Ready ready) {
   const int g4 = lane >> 2, t4 = lane & 3, R = A.T * A.places, steps = (A.I + STEP - 1) / STEP;
   const int per = (steps + splits - 1) / splits, total = ngroups * splits, kl = A.I - t4 * 8;
   int pt = warp, ps = 0, pend = 0;  // the task whose steps are being requested, its next step and the end of its range
-  const bf16 *ra = nullptr, *rb = nullptr, *xr[NF];
+  const bf16 *row = nullptr, *xr[NF];
   bool have[NF];
   Group<NF> next;
   if (pt < total) next.load(groups + pt / splits, g4);
-  const bool second = r0 + 8 < A.H;  // H is a multiple of 8: the last block may have 8 columns
+  const int pieces = min(2 * MT, (A.H - r0) / 8);  // H is a multiple of 8
   auto open = [&]() {
-    ra = A.w_d + next.e * A.d_e + static_cast<int64_t>(r0 + g4) * A.d_r + t4 * 8;
-    rb = second ? ra + 8 * A.d_r : ra;
+    row = A.w_d + next.e * A.d_e + static_cast<int64_t>(r0 + g4) * A.d_r + t4 * 8;
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
       xr[f] = A.h + static_cast<int64_t>(next.place[f]) * A.I + t4 * 8;
@@ -336,12 +361,12 @@ __device__ __forceinline__ void down_tasks(const MoeArgs& A, const G* groups, in
     if (ps >= pend) advance();
   }
   const int early = pt < total ? min(D, pend - ps) : 0;
-  for (int d = 0; d < early; ++d) q.weights(d, ra, rb, second, (ps + d) * STEP, kl);
+  for (int d = 0; d < early; ++d) q.weights(d, row, 16 * A.d_r, 8 * A.d_r, pieces, (ps + d) * STEP, kl);
   ready();
 #pragma unroll
   for (int d = 0; d < D; ++d) {
     if (pt < total) {
-      if (d >= early) q.weights(d, ra, rb, second, ps * STEP, kl);
+      if (d >= early) q.weights(d, row, 16 * A.d_r, 8 * A.d_r, pieces, ps * STEP, kl);
       q.rows(d, xr, have, ps * STEP, kl);
       advance();
     }
@@ -356,47 +381,47 @@ __device__ __forceinline__ void down_tasks(const MoeArgs& A, const G* groups, in
     for (int f = 0; f < NF; ++f)
 #pragma unroll
       for (int c = 0; c < 2; ++c) place[f][c] = f * 8 + t4 * 2 + c < n ? plan_load(gr, &gr->place[f * 8 + t4 * 2 + c]) : -1;
-    float acc[NF][4];
-#pragma unroll
-    for (int f = 0; f < NF; ++f)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) acc[f][c] = 0.f;
+    float acc[MT][NF][4];
+    clear(acc);
     for (int s = sp * per; s < min(steps, (sp + 1) * per); ++s) {
       q.pop(acc);
       if (pt < total) {
-        q.weights(q.put, ra, rb, second, ps * STEP, kl);
+        q.weights(q.put, row, 16 * A.d_r, 8 * A.d_r, pieces, ps * STEP, kl);
         q.rows(q.put, xr, have, ps * STEP, kl);
         advance();
       }
       q.pushed();
     }
-    float* v = val + static_cast<int64_t>(sp) * R * 16;
+    float* v = val + static_cast<int64_t>(sp) * R * 16 * MT + g4;
 #pragma unroll
     for (int f = 0; f < NF; ++f)
 #pragma unroll
       for (int c = 0; c < 2; ++c)
-        if (place[f][c] >= 0) {
-          v[place[f][c] * 16 + g4] = acc[f][c];
-          v[place[f][c] * 16 + g4 + 8] = acc[f][c + 2];
-        }
+        if (place[f][c] >= 0)
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            v[(place[f][c] * MT + m) * 16] = acc[m][f][c];
+            v[(place[f][c] * MT + m) * 16 + 8] = acc[m][f][c + 2];
+          }
   }
   copy_wait<0>();
   q.put = q.get = 0;
 }
 
 // The addend of this thread's first columns in down_sum, read before the products so that its latency passes meanwhile.
+template <int MT>
 __device__ __forceinline__ uint32_t down_addend(const MoeArgs& A, int r0) {
-  const int t = threadIdx.x >> 3, c = (threadIdx.x & 7) * 2;
+  const int t = threadIdx.x / (8 * MT), c = threadIdx.x % (8 * MT) * 2;
   return A.addend && t < A.T && r0 + c < A.H ? *reinterpret_cast<const uint32_t*>(A.addend + t * A.a_t + r0 + c) : 0u;
 }
 
 // Each token's places in their order, two columns a thread. have(p): whether place p has an expert, weight(p): its weight.
-template <typename Have, typename Weight>
+template <int MT, typename Have, typename Weight>
 __device__ __forceinline__ void down_sum(const MoeArgs& A, int splits, int r0, const float* val, uint32_t first, Have have,
                                          Weight weight) {
   const int R = A.T * A.places;
-  for (int j = threadIdx.x; j < A.T * 8; j += blockDim.x) {
-    const int t = j >> 3, c = (j & 7) * 2;
+  for (int j = threadIdx.x; j < A.T * 8 * MT; j += blockDim.x) {
+    const int t = j / (8 * MT), c = j % (8 * MT) * 2;
     if (r0 + c >= A.H) continue;
     if (j != static_cast<int>(threadIdx.x)) first = A.addend ? *reinterpret_cast<const uint32_t*>(A.addend + t * A.a_t + r0 + c) : 0u;
     float2 s = unpack_bf16x2(first);
@@ -405,7 +430,7 @@ __device__ __forceinline__ void down_sum(const MoeArgs& A, int splits, int r0, c
       const int p = t * A.places + k;
       float y0 = 0.f, y1 = 0.f;
       for (int sp = 0; sp < splits; ++sp) {
-        const float2 v = *reinterpret_cast<const float2*>(val + (static_cast<int64_t>(sp) * R + p) * 16 + c);
+        const float2 v = *reinterpret_cast<const float2*>(val + (static_cast<int64_t>(sp) * R + p) * 16 * MT + c);
         y0 += v.x;
         y1 += v.y;
       }
@@ -420,37 +445,37 @@ __device__ __forceinline__ void down_sum(const MoeArgs& A, int splits, int r0, c
 }
 
 // ------------------------------------------------------------------------------------------------ planned: two kernels
-template <int NF, int D>
+template <int MT, int NF, int D>
 constexpr int up_shared() {
-  return UP_WARPS * Queue<NF, D>::BYTES + UP_WARPS * NF * 512;
+  return UP_WARPS * Queue<MT, NF, D>::BYTES + UP_WARPS * MT * NF * 512;
 }
 
-template <int NF, int D>
-__global__ void __launch_bounds__(UP_WARPS * 32, NF == 1 ? 4 : 3) moe_up_few(const MoeArgs A) {
+template <int MT, int NF, int D>
+__global__ void __launch_bounds__(UP_WARPS * 32, NF == 1 ? 4 : 2) moe_up_few(const MoeArgs A) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  Queue<NF, D> q;
-  q.base = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * Queue<NF, D>::BYTES + lane * 16;
+  Queue<MT, NF, D> q;
+  q.base = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * Queue<MT, NF, D>::BYTES + lane * 16;
   pdl_wait();
   pdl_trigger();  // after the wait: what was planned is then visible to the next kernel before its own wait
-  up_units<NF, D>(A, A.groups, __ldcg(&A.header->ngroups), blockIdx.x, gridDim.x, warp, lane, q,
-                  reinterpret_cast<float4*>(smem + UP_WARPS * Queue<NF, D>::BYTES), []() { __syncthreads(); });
+  up_units(A, A.groups, __ldcg(&A.header->ngroups), blockIdx.x, gridDim.x, warp, lane, q,
+           reinterpret_cast<float4*>(smem + UP_WARPS * Queue<MT, NF, D>::BYTES), []() { __syncthreads(); });
 }
 
 // Shared memory: the queues, the places' results, their weights and whether they have an expert.
-template <int WARPS, int NF, int D>
+template <int WARPS, int MT, int NF, int D>
 constexpr int down_shared(int R, int splits) {
-  return WARPS * Queue<NF, D>::BYTES + R * (64 * splits + 8);
+  return WARPS * Queue<MT, NF, D>::BYTES + R * (64 * MT * splits + 8);
 }
 
-// Block b: output columns 16 b .. 16 b + 15 of every token.
-template <int WARPS, int NF, int D>
+// Block b: output columns 16 MT b .. of every token.
+template <int WARPS, int MT, int NF, int D>
 __global__ void __launch_bounds__(WARPS * 32) moe_down_few(const MoeArgs A, int max_splits) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int R = A.T * A.places, r0 = blockIdx.x * 16;
-  float* val = reinterpret_cast<float*>(smem + WARPS * Queue<NF, D>::BYTES);  // [split][place][16]
-  float* s_w = val + static_cast<int64_t>(max_splits) * R * 16;
+  const int R = A.T * A.places, r0 = blockIdx.x * 16 * MT;
+  float* val = reinterpret_cast<float*>(smem + WARPS * Queue<MT, NF, D>::BYTES);  // [split][place][16 MT]
+  float* s_w = val + static_cast<int64_t>(max_splits) * R * 16 * MT;
   int* s_ok = reinterpret_cast<int*>(s_w + R);
   // the plan is complete: the kernel before this one let it start only after its own wait for it
   const int ngroups = __ldcg(&A.header->ngroups);
@@ -460,16 +485,16 @@ __global__ void __launch_bounds__(WARPS * 32) moe_down_few(const MoeArgs A, int 
     s_ok[p] = e >= 0 && e < A.E;
   }
   const int splits = down_splits(ngroups, (A.I + STEP - 1) / STEP, WARPS, max_splits, lane);
-  Queue<NF, D> q;
-  q.base = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * Queue<NF, D>::BYTES + lane * 16;
+  Queue<MT, NF, D> q;
+  q.base = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * Queue<MT, NF, D>::BYTES + lane * 16;
   uint32_t first = 0;
-  down_tasks<NF, D>(A, A.groups, ngroups, splits, r0, warp, WARPS, lane, q, val, [&]() {
+  down_tasks(A, A.groups, ngroups, splits, r0, warp, WARPS, lane, q, val, [&]() {
     pdl_wait();
-    first = down_addend(A, r0);
+    first = down_addend<MT>(A, r0);
   });
   pdl_trigger();
   __syncthreads();
-  down_sum(A, splits, r0, val, first, [=](int p) { return s_ok[p] != 0; }, [=](int p) { return s_w[p]; });
+  down_sum<MT>(A, splits, r0, val, first, [=](int p) { return s_ok[p] != 0; }, [=](int p) { return s_w[p]; });
 }
 
 // ------------------------------------------------------------------------------------------------ tiny: one kernel
@@ -477,18 +502,18 @@ __global__ void __launch_bounds__(WARPS * 32) moe_down_few(const MoeArgs A, int 
 // for itself; four crews of 8 warps take up units; then every warp requests its first down weights and the grid meets; then
 // all 32 warps take down tasks. 1 token x 9 of 257 experts (H 2048, I 512): as two launches 24.7 us.
 constexpr int TINY_WARPS = 32, TINY_D = 2, TINY_RED = TINY_WARPS * 512;
-constexpr int TINY_SHARED = TINY_WARPS * Queue<1, TINY_D>::BYTES + TINY_RED + static_cast<int>(sizeof(TinyPlan));
+constexpr int TINY_SHARED = TINY_WARPS * Queue<1, 1, TINY_D>::BYTES + TINY_RED + static_cast<int>(sizeof(TinyPlan));
 
 template <int V, bool F32>
 __global__ void __launch_bounds__(TINY_WARPS * 32, 1) moe_tiny(const MoeArgs A, const RouteParams P) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, crew = warp / UP_WARPS;
-  uint8_t* red = smem + TINY_WARPS * Queue<1, TINY_D>::BYTES;  // up: the crews' partial sums; down: the places' results
+  uint8_t* red = smem + TINY_WARPS * Queue<1, 1, TINY_D>::BYTES;  // up: the crews' partial sums; down: the places' results
   TinyPlan& S = *reinterpret_cast<TinyPlan*>(red + TINY_RED);
-  Queue<1, TINY_D> q;
-  q.base = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * Queue<1, TINY_D>::BYTES + lane * 16;
+  Queue<1, 1, TINY_D> q;
+  q.base = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * Queue<1, 1, TINY_D>::BYTES + lane * 16;
   tiny_plan<V, F32>(A, P, S, blockIdx.x == 0);
-  up_units<1, TINY_D>(A, S.g, S.ngroups, blockIdx.x + gridDim.x * crew, gridDim.x * (TINY_WARPS / UP_WARPS), warp % UP_WARPS, lane, q,
+  up_units(A, S.g, S.ngroups, blockIdx.x + gridDim.x * crew, gridDim.x * (TINY_WARPS / UP_WARPS), warp % UP_WARPS, lane, q,
                       reinterpret_cast<float4*>(red + crew * UP_WARPS * 512),
                       [=]() { asm volatile("bar.sync %0, %1;\n" ::"r"(crew + 1), "n"(UP_WARPS * 32) : "memory"); });
   const int R = A.T * A.places, tiles = (A.H + 15) / 16;
@@ -504,10 +529,10 @@ __global__ void __launch_bounds__(TINY_WARPS * 32, 1) moe_tiny(const MoeArgs A, 
       meet();
       break;
     }
-    const uint32_t first = down_addend(A, tile * 16);
-    down_tasks<1, TINY_D>(A, S.g, S.ngroups, splits, tile * 16, warp, TINY_WARPS, lane, q, val, meet);
+    const uint32_t first = down_addend<1>(A, tile * 16);
+    down_tasks(A, S.g, S.ngroups, splits, tile * 16, warp, TINY_WARPS, lane, q, val, meet);
     __syncthreads();
-    down_sum(A, splits, tile * 16, val, first, [&](int p) { return S.id[p] >= 0; }, [&](int p) { return S.w[p]; });
+    down_sum<1>(A, splits, tile * 16, val, first, [&](int p) { return S.id[p] >= 0; }, [&](int p) { return S.w[p]; });
     __syncthreads();  // the results are overwritten next
   }
 }
@@ -548,53 +573,56 @@ int launch_tiny(const MoeArgs& A, const RouteParams& P, int sms, cudaStream_t s)
   return mmp_check_launch("mmp_moe_experts");
 }
 
-template <int NF>
+template <int MT, int NF>
 int launch_up(const MoeArgs& A, int max_groups, int sms, cudaStream_t s) {
-  constexpr int D = 2, bytes = up_shared<NF, D>();
-  auto kern = moe_up_few<NF, D>;
+  constexpr int D = 2, bytes = up_shared<MT, NF, D>();
+  auto kern = moe_up_few<MT, NF, D>;
   static bool set[64] = {};
   int rc = allow_shared(kern, bytes, set);
   if (rc != MMP_OK) return rc;
-  constexpr int per_sm = std::min(NF == 1 ? 4 : 3, SM_SHARED / (bytes + 1024));
-  const int64_t units = static_cast<int64_t>(max_groups) * (A.I / 8);
+  constexpr int per_sm = std::min(NF == 1 ? 4 : 2, SM_SHARED / (bytes + 1024));
+  const int64_t units = static_cast<int64_t>(max_groups) * ((A.I + 8 * MT - 1) / (8 * MT));
   const int grid = static_cast<int>(std::min<int64_t>(units, static_cast<int64_t>(sms) * per_sm));
   cudaError_t e = launch_kind(1, kern, dim3(grid), dim3(UP_WARPS * 32), bytes, s, nullptr, 0, A);
   if (e != cudaSuccess) return mmp_set_error(MMP_ERR_CUDA, "mmp_moe_experts: %s", cudaGetErrorString(e));
   return MMP_OK;
 }
 
-template <int WARPS, int NF, int D>
+template <int WARPS, int MT, int NF, int D>
 int launch_down(const MoeArgs& A, int limit, cudaStream_t s) {
-  auto kern = moe_down_few<WARPS, NF, D>;
+  auto kern = moe_down_few<WARPS, MT, NF, D>;
   static bool set[64] = {};
   int rc = allow_shared(kern, SM_SHARED, set);
   if (rc != MMP_OK) return rc;
   const int R = A.T * A.places;
   int splits = 1;
-  while (splits < WARPS && down_shared<WARPS, NF, D>(R, splits + 1) <= limit) ++splits;
-  cudaError_t e = launch_kind(1, kern, dim3((A.H + 15) / 16), dim3(WARPS * 32), down_shared<WARPS, NF, D>(R, splits), s, nullptr, 0, A,
-                              splits);
+  while (splits < WARPS && down_shared<WARPS, MT, NF, D>(R, splits + 1) <= limit) ++splits;
+  cudaError_t e = launch_kind(1, kern, dim3((A.H + 16 * MT - 1) / (16 * MT)), dim3(WARPS * 32),
+                              down_shared<WARPS, MT, NF, D>(R, splits), s, nullptr, 0, A, splits);
   if (e != cudaSuccess) return mmp_set_error(MMP_ERR_CUDA, "mmp_moe_experts: %s", cudaGetErrorString(e));
   return MMP_OK;
 }
 
-static_assert(down_shared<8, 2, 2>(MOE_FEW_PLACES, 1) <= SM_SHARED, "the last choice of products() takes any request");
+// 16 warps while one block an SM covers the columns, else two blocks of 8; as long a queue as fits beside the results.
+static_assert(down_shared<8, 1, 2, 2>(MOE_FEW_PLACES, 1) <= SM_SHARED && down_shared<8, 1, 1, 2>(MOE_FEW_PLACES, 1) <= SM_SHARED,
+              "the last choices take any request");
 
-template <int NF>
-int products(const MoeArgs& A, int max_groups, int sms, cudaStream_t s) {
-  int rc = launch_up<NF>(A, max_groups, sms, s);
+int products8(const MoeArgs& A, int max_groups, int sms, cudaStream_t s) {
+  int rc = launch_up<1, 1>(A, max_groups, sms, s);
   if (rc != MMP_OK) return rc;
-  // 16 warps while one block an SM covers the columns, else two blocks of 8; as long a queue as fits beside the results
-  const int R = A.T * A.places;
-  if ((A.H + 15) / 16 <= sms) {
-    if (down_shared<16, NF, 3>(R, 1) <= SM_SHARED) rc = launch_down<16, NF, 3>(A, SM_SHARED, s);
-    else rc = launch_down<8, NF, 2>(A, SM_SHARED, s);
-  } else {
-    const int half = SM_SHARED / 2 - 1024;
-    if (down_shared<8, NF, 3>(R, 1) <= half) rc = launch_down<8, NF, 3>(A, half, s);
-    else rc = launch_down<8, NF, 2>(A, SM_SHARED, s);
-  }
-  return rc != MMP_OK ? rc : mmp_check_launch("mmp_moe_experts");
+  const int R = A.T * A.places, half = SM_SHARED / 2 - 1024;
+  if ((A.H + 15) / 16 <= sms && down_shared<16, 1, 1, 3>(R, 1) <= SM_SHARED) return launch_down<16, 1, 1, 3>(A, SM_SHARED, s);
+  if ((A.H + 15) / 16 > sms && down_shared<8, 1, 1, 3>(R, 1) <= half) return launch_down<8, 1, 1, 3>(A, half, s);
+  return launch_down<8, 1, 1, 2>(A, SM_SHARED, s);
+}
+
+int products16(const MoeArgs& A, int max_groups, int sms, cudaStream_t s) {
+  int rc = launch_up<2, 2>(A, max_groups, sms, s);
+  if (rc != MMP_OK) return rc;
+  const int R = A.T * A.places, half = SM_SHARED / 2 - 1024;
+  if ((A.H + 31) / 32 <= sms && down_shared<16, 2, 2, 2>(R, 1) <= SM_SHARED) return launch_down<16, 2, 2, 2>(A, SM_SHARED, s);
+  if (down_shared<8, 2, 2, 2>(R, 1) <= half) return launch_down<8, 2, 2, 2>(A, half, s);
+  return launch_down<8, 1, 2, 2>(A, SM_SHARED, s);
 }
 
 }  // namespace
@@ -611,7 +639,8 @@ int moe_products_few(const MoeArgs& A, const RouteParams& P, bool f32, const Moe
     return f32 ? launch_tiny<32, true>(A, P, sms, s) : launch_tiny<32, false>(A, P, sms, s);
   }
   const int R = A.T * A.places, most = std::min(R, R / plan.rows + A.E);
-  return plan.rows == 8 ? products<1>(A, most, sms, s) : products<2>(A, most, sms, s);
+  const int rc = plan.rows == 8 ? products8(A, most, sms, s) : products16(A, most, sms, s);
+  return rc != MMP_OK ? rc : mmp_check_launch("mmp_moe_experts");
 }
 
 }  // namespace mmp
