@@ -397,6 +397,8 @@ int mmp_gdn_prefill_tc(const void* q, int64_t q_t, int64_t q_h, const void* k, i
 int mmp_moe_route(const void* logits, int logits_dtype, int64_t l_t, int T, int E, int top_k, int renormalize, int shared,
                   float* weights, int32_t* ids, void* stream);
 size_t mmp_moe_workspace_size(int T, int places, int H, int I, int E);
+/* Kernels that one mmp_moe_experts (route 0) or mmp_moe_layer (route 1) of these sizes launches. */
+int mmp_moe_launches(int T, int places, int H, int I, int E, int route);
 int mmp_moe_experts(const void* x, int64_t x_t, const void* w_gate_up, int64_t gu_e, int64_t gu_r, const void* w_down,
                     int64_t d_e, int64_t d_r, const float* weights, int64_t w_t, const int32_t* ids, int64_t id_t,
                     const void* addend, int64_t a_t, void* out, int64_t o_t, int T, int places, int H, int I, int E,

@@ -38,6 +38,7 @@ SIGNATURES: dict[str, tuple] = {
                                  I32, P, I32, P, P]),
     "mmp_moe_route": (I32, [P, I32, I64, I32, I32, I32, I32, I32, P, P, P]),
     "mmp_moe_workspace_size": (SZ, [I32, I32, I32, I32, I32]),
+    "mmp_moe_launches": (I32, [I32, I32, I32, I32, I32, I32]),
     "mmp_moe_experts": (I32, [P, I64, P, I64, I64, P, I64, I64, P, I64, P, I64, P, I64, P, I64, I32, I32, I32, I32, I32,
                               P, SZ, P, P]),
     "mmp_moe_layer": (I32, [P, I64, P, I32, I64, P, I64, I64, P, I64, I64, P, I64, P, I64, I32, I32, I32, I32, I32, I32,

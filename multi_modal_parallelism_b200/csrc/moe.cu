@@ -151,7 +151,7 @@ __global__ void __cluster_dims__(PLAN_BLOCKS, 1, 1) __launch_bounds__(1024) moe_
       n += c;
       before += b < me ? c : 0;
     }
-  const int nb = (n + MOE_BLOCK_ROWS - 1) / MOE_BLOCK_ROWS;
+  const int nb = (n + A.block_rows - 1) / A.block_rows;
   int2 total;
   const int2 pre = scan_block(make_int2(n, nb), warp_tot, total);
   const int off = pre.x;
@@ -186,6 +186,7 @@ __global__ void __launch_bounds__(256) moe_sort_rows(const MoeArgs A) {
 // ------------------------------------------------------------------------------------------------ weighted sum
 // out_t = addend_t + sum_k w_{t,k} y[pos_{t,k}]: block (token), eight columns a thread.
 __global__ void __launch_bounds__(256) moe_combine(const MoeArgs A) {
+  pdl_wait();
   const int t = blockIdx.x;
   const int64_t tt = t;
   for (int c = threadIdx.x * 8; c < A.H; c += 256 * 8) {
@@ -236,13 +237,14 @@ struct LaunchPlan {
   }
 };
 
+constexpr int FUSED_ROUTE_TOKENS = 32;  // a warp of the planning block a token; more are routed by a launch over the GPU
+
 // The few-token kernels; P.logits set: routing from the logits, else the ids are given.
 int few_products(const MoeArgs& A, const RouteParams& P, bool f32, cudaStream_t s) {
   const MoeFewPlan plan = moe_few_plan(A);
   if (plan.tiny) return moe_products_few(A, P, f32, plan, s);
   int rc = MMP_OK;
-  // a warp of the planning block a token; more tokens are routed by a launch over the GPU
-  if (P.logits && A.T <= 32) {
+  if (P.logits && A.T <= FUSED_ROUTE_TOKENS) {
     rc = by_width<LaunchPlan>(P.E, f32, A, P, plan.rows, s);
   } else {
     if (P.logits) rc = by_width<LaunchRoute>(P.E, f32, P, s);
@@ -253,14 +255,16 @@ int few_products(const MoeArgs& A, const RouteParams& P, bool f32, cudaStream_t 
   return rc != MMP_OK ? rc : moe_products_few(A, P, f32, plan, s);
 }
 
-int many_products(const MoeArgs& A, const MoeLayout& L, cudaStream_t s) {
+int many_products(MoeArgs& A, const MoeLayout& L, cudaStream_t s) {
+  A.block_rows = static_cast<int64_t>(A.T) * A.places <= 64 * A.E ? MOE_BLOCK_ROWS_FEW : MOE_BLOCK_ROWS;
   cudaError_t e = launch_kind(1, moe_plan_many, dim3(PLAN_BLOCKS), dim3(1024), 0, s, nullptr, 0, A);
   if (e != cudaSuccess) return mmp_set_error(MMP_ERR_CUDA, "mmp_moe_experts: %s", cudaGetErrorString(e));
   e = launch_kind(1, moe_sort_rows, dim3(A.T), dim3(256), 0, s, nullptr, 0, A);
   if (e != cudaSuccess) return mmp_set_error(MMP_ERR_CUDA, "mmp_moe_experts: %s", cudaGetErrorString(e));
   const int rc = moe_products_tc(A, L.max_blocks, s);
   if (rc != MMP_OK) return rc;
-  moe_combine<<<A.T, 256, 0, s>>>(A);
+  e = launch_kind(1, moe_combine, dim3(A.T), dim3(256), 0, s, nullptr, 0, A);
+  if (e != cudaSuccess) return mmp_set_error(MMP_ERR_CUDA, "mmp_moe_experts: %s", cudaGetErrorString(e));
   return mmp_check_launch("mmp_moe_experts");
 }
 
@@ -327,6 +331,17 @@ extern "C" size_t mmp_moe_workspace_size(int T, int places, int H, int I, int E)
   return moe_layout(T, places, H, I, E).bytes;
 }
 
+extern "C" int mmp_moe_launches(int T, int places, int H, int I, int E, int route) {
+  if (T <= 0 || places <= 0 || H <= 0 || I <= 0 || E <= 0) return 0;
+  if (!moe_is_few(T, places, H, I, E)) return 5 + (route ? 1 : 0);  // plan, sorted rows, up, down, sum; routing
+  MoeArgs A{};
+  A.T = T;
+  A.places = places;
+  A.E = E;
+  if (moe_few_plan(A).tiny) return 1;
+  return 3 + (route && T > FUSED_ROUTE_TOKENS ? 1 : 0);  // plan (with the routing of few tokens), up, down
+}
+
 extern "C" int mmp_moe_experts(const void* x, int64_t x_t, const void* w_gate_up, int64_t gu_e, int64_t gu_r, const void* w_down,
                                int64_t d_e, int64_t d_r, const float* weights, int64_t w_t, const int32_t* ids, int64_t id_t,
                                const void* addend, int64_t a_t, void* out, int64_t o_t, int T, int places, int H, int I, int E,
@@ -343,7 +358,7 @@ extern "C" int mmp_moe_experts(const void* x, int64_t x_t, const void* w_gate_up
     return mmp_set_error(MMP_ERR_INVALID, "mmp_moe_experts: weights and ids must be [T, places]");
   place_workspace(A, L, workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return moe_is_few(T, places, E) ? few_products(A, RouteParams{}, false, s) : many_products(A, L, s);
+  return moe_is_few(T, places, H, I, E) ? few_products(A, RouteParams{}, false, s) : many_products(A, L, s);
 }
 
 extern "C" int mmp_moe_layer(const void* x, int64_t x_t, const void* logits, int logits_dtype, int64_t l_t, const void* w_gate_up,
@@ -367,7 +382,7 @@ extern "C" int mmp_moe_layer(const void* x, int64_t x_t, const void* logits, int
   A.ids = ids;
   RouteParams P{logits, l_t, T, routed, top_k, renormalize ? 1 : 0, shared ? 1 : 0, w, ids};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (moe_is_few(T, places, E)) return few_products(A, P, logits_dtype == MMP_F32, s);
+  if (moe_is_few(T, places, H, I, E)) return few_products(A, P, logits_dtype == MMP_F32, s);
   rc = by_width<LaunchRoute>(routed, logits_dtype == MMP_F32, P, s);
   return rc != MMP_OK ? rc : many_products(A, L, s);
 }

@@ -15,7 +15,9 @@ constexpr int MOE_MAX_EXPERTS = 1024;  // experts in the weight tensors (one thr
 constexpr int MOE_MAX_TOPK = 32;       // one lane each in the router
 constexpr int MOE_FEW_PLACES = 1536;   // the few-token kernels keep 16 fp32 a place in shared memory (96 KB)
 constexpr int MOE_TINY_TOKENS = 8, MOE_TINY_PLACES = 64;  // up to which every block of the few-token kernels plans for itself
-constexpr int MOE_BLOCK_ROWS = 256;    // sorted rows of one expert that the tensor-core kernels take at a time (MMA N)
+// Sorted rows of one expert that the tensor-core kernels take at a time (MMA N): 256, or 128 with a deeper ring of weights
+// where experts have few rows.
+constexpr int MOE_BLOCK_ROWS = 256, MOE_BLOCK_ROWS_FEW = 128;
 
 struct MoeHeader {
   int ngroups;  // groups of the few-token kernels
@@ -29,7 +31,15 @@ struct MoeGroup {
   int place[16];
 };
 
-inline bool moe_is_few(int64_t T, int places, int E) { return T * places <= MOE_FEW_PLACES; }
+// The few-token kernels where experts have few rows, the tensor-core kernels else. Measured (us, few-token / tensor-core):
+// 576 places on 257 experts of 6.3 MB 222 / 225, 1152 places 327 / 268; 32 on 8 of 176 MB 299 / 254; 256 on 60 of 17 MB
+// 205 / 174. Where the experts together are small the latter's five launches weigh more: 64 places on 8 of 6.3 MB 20 / 32,
+// 256 on 60 of 3.1 MB 47 / 55, 512 on 16 of 1.6 MB 29 / 26.
+inline bool moe_is_few(int64_t T, int places, int H, int I, int E) {
+  const int64_t R = T * places;
+  if (R > MOE_FEW_PLACES) return false;
+  return 2 * R <= 5 * E || (R <= 12 * E && 6LL * E * H * I <= 200000000);
+}
 
 // Workspace offsets in bytes, every part 256-byte aligned.
 struct MoeLayout {
@@ -42,9 +52,9 @@ inline size_t moe_align(size_t n) { return (n + 255) / 256 * 256; }
 inline MoeLayout moe_layout(int64_t T, int places, int H, int I, int E) {
   MoeLayout L;
   const int64_t R = T * places;
-  const bool few = moe_is_few(T, places, E);
+  const bool few = moe_is_few(T, places, H, I, E);
   // the sum over experts of ceil(n / b) is at most R / b + E, and R
-  L.max_blocks = static_cast<int>(std::min<int64_t>(R, R / MOE_BLOCK_ROWS + E));
+  L.max_blocks = static_cast<int>(std::min<int64_t>(R, R / MOE_BLOCK_ROWS_FEW + E));
   size_t at = 0;
   auto part = [&](size_t n) { const size_t o = at; at += moe_align(n); return o; };
   L.header = part(sizeof(MoeHeader));
@@ -71,6 +81,7 @@ struct MoeArgs {
   const bf16* addend; int64_t a_t;
   bf16* out; int64_t o_t;
   int T, places, H, I, E;
+  int block_rows;  // tensor-core path
   MoeHeader* header;
   MoeGroup* groups;
   int4* blocks;   // {expert, its first sorted row, its rows, index among its blocks} of the row blocks

@@ -25,10 +25,10 @@ namespace {
 
 constexpr int MK = 64, MTHREADS = 192;
 
-template <int STAGES>
+template <int STAGES, int ROWS>
 struct MLayout {
   static constexpr int A_BYTES = 128 * MK * 2;                  // this block's 128 weight rows
-  static constexpr int B_BYTES = MOE_BLOCK_ROWS / 2 * MK * 2;   // its half of the rows
+  static constexpr int B_BYTES = ROWS / 2 * MK * 2;             // its half of the rows
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int BARS = STAGES * STAGE_BYTES;  // full[S], empty[S], acc_full[2], acc_empty[2]
   static constexpr int TMEM_SLOT = BARS + 8 * (2 * STAGES + 4);
@@ -78,7 +78,7 @@ struct Item { int expert, row0, n, tile; };
 __device__ __forceinline__ Item moe_item(const MoeArgs& A, int it, int tiles) {
   const int b = it / tiles;
   const int4 r = __ldcg(A.blocks + b);
-  const int nb = (r.z + MOE_BLOCK_ROWS - 1) / MOE_BLOCK_ROWS, q = it - (b - r.w) * tiles, tile = q / nb, j = q - tile * nb;
+  const int nb = (r.z + A.block_rows - 1) / A.block_rows, q = it - (b - r.w) * tiles, tile = q / nb, j = q - tile * nb;
   // blocks of nearly equal size
   const int r0 = static_cast<int>(static_cast<int64_t>(r.z) * j / nb), r1 = static_cast<int>(static_cast<int64_t>(r.z) * (j + 1) / nb);
   return {r.x, r.y + r0, r1 - r0, tile};
@@ -86,10 +86,10 @@ __device__ __forceinline__ Item moe_item(const MoeArgs& A, int it, int tiles) {
 
 // Two blocks of a cluster are a pair on one 256-row tile: each loads its 128 weight rows and half of the block's rows of B,
 // the leader (rank 0) issues the MMAs for both (cta_group::2), each drains its own 128 rows of the accumulator.
-template <bool UP, int STAGES>
+template <bool UP, int STAGES, int ROWS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
     moe_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const MoeArgs A, int tiles) {
-  using L = MLayout<STAGES>;
+  using L = MLayout<STAGES, ROWS>;
   extern __shared__ uint8_t dsmem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_addr(smem);
@@ -127,14 +127,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
   pair_sync();  // both blocks' barriers are set up and their TMEM is allocated
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_wait();
-  pdl_trigger();
+  // The plan is complete: the kernel before this one let it start only after its own wait for it. Warp 0 requests its first
+  // weights before it waits for what that kernel writes, the rows of B.
   const int nitems = __ldcg(&A.header->nblk) * tiles;
+  if (warp != 0) {
+    pdl_wait();
+    pdl_trigger();
+  }
 
   int issued = 0;  // stages requested by warp 0 (drained at teardown after an abort)
   if (warp == 0) {
-    int kc = 0;
+    int kc = 0, early = 0;
     bool ok = true;
+    if (pair < nitems) {
+      const Item blk = moe_item(A, pair, tiles);
+      const int tile = blk.tile * 2 + rank;
+      early = min(k_tiles, STAGES);
+      if (lane == 0)
+        for (int kt = 0; kt < early; ++kt) {
+          const uint32_t a_s = sbase + kt * L::STAGE_BYTES, bar = mapa(full_bar(kt), 0);
+          if (UP) pair_load_5d(a_s, &tmA, bar, kt * MK, 0, 0, tile * 8, blk.expert);
+          else pair_load_3d(a_s, &tmA, bar, kt * MK, tile * 128, blk.expert);
+        }
+    }
+    __syncwarp();
+    pdl_wait();
+    pdl_trigger();
     for (int it = pair; it < nitems && ok; it += npairs) {
       const Item blk = moe_item(A, it, tiles);
       const int tile = blk.tile * 2 + rank;
@@ -154,8 +172,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
         const uint32_t bar = mapa(full_bar(s), 0);  // the leader's; bytes may arrive there before they are announced
         if (lane == 0) {
           if (rank == 0) mbar_expect_tx(full_bar(s), bytes);
-          if (UP) pair_load_5d(a_s, &tmA, bar, kt * MK, 0, 0, tile * 8, blk.expert);
-          else pair_load_3d(a_s, &tmA, bar, kt * MK, tile * 128, blk.expert);
+          if (kc >= early) {
+            if (UP) pair_load_5d(a_s, &tmA, bar, kt * MK, 0, 0, tile * 8, blk.expert);
+            else pair_load_3d(a_s, &tmA, bar, kt * MK, tile * 128, blk.expert);
+          }
         }
         if (lane < nb) pair_load_2d(b_s + lane * 64 * MK * 2, &tmB, bar, kt * MK, blk.row0 + static_cast<int>(rank) * half + lane * 64);
         ++issued;
@@ -260,11 +280,10 @@ int encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims,
   return MMP_OK;
 }
 
-template <bool UP>
+template <bool UP, int STAGES, int ROWS>
 int launch_products(const CUtensorMap& ma, const CUtensorMap& mb, const MoeArgs& A, int tiles, int max_blocks, int sms, cudaStream_t s) {
-  constexpr int STAGES = 6;
-  using L = MLayout<STAGES>;
-  auto kern = moe_tc_kernel<UP, STAGES>;
+  using L = MLayout<STAGES, ROWS>;
+  auto kern = moe_tc_kernel<UP, STAGES, ROWS>;
   static bool set[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -315,8 +334,14 @@ int moe_products_tc(const MoeArgs& A, int max_blocks, cudaStream_t s) {
     const u32 box[2] = {MK, 64};
     if ((rc = encode(&mh, A.h, 2, dims, strides, box)) != MMP_OK) return rc;
   }
-  if ((rc = launch_products<true>(mgu, mx, A, (A.I + 127) / 128, max_blocks, sms, s)) != MMP_OK) return rc;
-  if ((rc = launch_products<false>(md, mh, A, (A.H + 255) / 256, max_blocks, sms, s)) != MMP_OK) return rc;
+  const int up = (A.I + 127) / 128, down = (A.H + 255) / 256;
+  if (A.block_rows == MOE_BLOCK_ROWS_FEW) {
+    if ((rc = launch_products<true, 9, MOE_BLOCK_ROWS_FEW>(mgu, mx, A, up, max_blocks, sms, s)) != MMP_OK) return rc;
+    if ((rc = launch_products<false, 9, MOE_BLOCK_ROWS_FEW>(md, mh, A, down, max_blocks, sms, s)) != MMP_OK) return rc;
+  } else {
+    if ((rc = launch_products<true, 6, MOE_BLOCK_ROWS>(mgu, mx, A, up, max_blocks, sms, s)) != MMP_OK) return rc;
+    if ((rc = launch_products<false, 6, MOE_BLOCK_ROWS>(md, mh, A, down, max_blocks, sms, s)) != MMP_OK) return rc;
+  }
   return mmp_check_launch("mmp_moe_experts");
 }
 

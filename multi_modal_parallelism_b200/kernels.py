@@ -728,18 +728,6 @@ def gdn_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, a: torch.Tens
 
 
 # ----------------------------------------------------------------------------- mixture of experts
-def _moe_launches(T: int, places: int, route: bool) -> int:
-    """Kernels of one call (the library's rules on sizes)."""
-    n = T * places
-    if n == 0:
-        return 0
-    if T <= 8 and n <= 64:
-        return 1  # one cooperative launch
-    if n <= 1536:
-        return 3 + (route and T > 32)  # plan (with the routing of up to 32 tokens), up, down
-    return 5 + route  # plan, sorted rows, up, down, sum
-
-
 _LOGITS = {torch.float32: MMP_F32, BF16: MMP_BF16}
 
 
@@ -782,9 +770,14 @@ def moe_route(logits: torch.Tensor, top_k: int, weights: torch.Tensor | None = N
     return weights, ids
 
 
-@functools.lru_cache(maxsize=256)
+@functools.lru_cache(maxsize=1024)
 def _moe_workspace_bytes(T: int, places: int, hidden: int, intermediate: int, experts: int) -> int:
     return max(256, _lib.lib().mmp_moe_workspace_size(T, places, hidden, intermediate, experts))
+
+
+@functools.lru_cache(maxsize=1024)
+def _moe_launches(T: int, places: int, hidden: int, intermediate: int, experts: int, route: bool) -> int:
+    return _lib.lib().mmp_moe_launches(T, places, hidden, intermediate, experts, int(route))
 
 
 def moe_workspace(T: int, places: int, hidden: int, intermediate: int, experts: int, device: torch.device) -> torch.Tensor:
@@ -843,7 +836,7 @@ def moe_experts(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, 
     T, H, I, E, x_t, w, io, out, ws, n = _moe_args(name, x, w_gate_up, w_down, addend, out, workspace, places)
     err, stream = _err_and_stream(d, x)
     _call_on(d, "mmp_moe_experts", x.data_ptr(), x_t, *w, weights.data_ptr(), w_t, ids.data_ptr(), id_t, *io, T, places, H, I, E,
-             ws.data_ptr(), n, err, stream, kernels=_moe_launches(T, places, False))
+             ws.data_ptr(), n, err, stream, kernels=_moe_launches(T, places, H, I, E, False))
     return out
 
 
@@ -866,5 +859,5 @@ def moe_layer(x: torch.Tensor, logits: torch.Tensor, w_gate_up: torch.Tensor, w_
         raise ValueError(f"{name}: logits {tuple(logits.shape)} is not [{T}, {E}]")
     err, stream = _err_and_stream(d, x)
     _call_on(d, "mmp_moe_layer", x.data_ptr(), x_t, logits.data_ptr(), dt, l_t, *w, *io, T, top_k, 1 if renormalize else 0, sh, H, I,
-             E, ws.data_ptr(), n, err, stream, kernels=_moe_launches(T, places, True))
+             E, ws.data_ptr(), n, err, stream, kernels=_moe_launches(T, places, H, I, E, True))
     return out

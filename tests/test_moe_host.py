@@ -107,8 +107,7 @@ def test_empty_batches_return_without_a_launch(cpu):
 def test_workspace_size_grows_with_the_request():
     size = lambda *a: _lib.lib().mmp_moe_workspace_size(*a)  # noqa: E731
     assert size(0, 2, 64, 32, 8) == 0
-    for a, b in (((4, 2, 64, 32, 8), (5, 2, 64, 32, 8)), ((768, 2, 64, 32, 8), (769, 2, 64, 32, 8))):
-        assert 0 < size(*a) <= size(*b)
+    assert 0 < size(4, 2, 64, 32, 8) <= size(5, 2, 64, 32, 8)
     R = 1000 * 2  # a large request holds the fp32 results and the bf16 intermediate rows
     assert size(1000, 2, 64, 32, 8) >= R * (64 * 4 + 32 * 2)
     # 64-bit sizes: 2^25 places of 8192 columns
