@@ -58,7 +58,8 @@ inline MoeLayout moe_layout(int64_t T, int places, int H, int I, int E) {
   size_t at = 0;
   auto part = [&](size_t n) { const size_t o = at; at += moe_align(n); return o; };
   L.header = part(sizeof(MoeHeader));
-  L.groups = part(few ? std::min<size_t>(R, R / 8 + E) * sizeof(MoeGroup) : 0);
+  const int64_t r = std::min<int64_t>(R, MOE_FEW_PLACES);  // there for more places too: a larger request's scratch serves a smaller one
+  L.groups = part(std::min<size_t>(r, r / 8 + E) * sizeof(MoeGroup));
   L.blocks = part(few ? 0 : static_cast<size_t>(L.max_blocks) * 16);
   L.rows = part(few ? 0 : R * 4);
   L.pos = part(few ? 0 : R * 4);

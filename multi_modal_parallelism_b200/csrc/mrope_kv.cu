@@ -122,7 +122,7 @@ extern "C" int mmp_mrope_kv_write(const void* qkv, int64_t row, int nq, int nkv,
   if (T == 0) return MMP_OK;
   if (!qkv || !positions || !inv_freq || !axes || !q_out || !key_cache || !value_cache || !slot_mapping)
     return mmp_set_error(MMP_ERR_INVALID, "mmp_mrope_kv_write: null pointer");
-  if ((T > 1 && (row < static_cast<int64_t>(nq + 2 * nkv) * hd || qo_b < static_cast<int64_t>(nq) * hd)) || (naxes > 1 && p_a < T))
+  if ((T > 1 && (row < static_cast<int64_t>(nq + 2 * nkv) * hd || qo_b < static_cast<int64_t>(nq) * hd)) || p_a < 0)
     return mmp_set_error(MMP_ERR_INVALID, "mmp_mrope_kv_write: rows overlap");
   MropeParams P{static_cast<const bf16*>(qkv), row, nq, nkv, hd, rd / 2, naxes, positions, p_a, inv_freq, axes, key_mult,
                 static_cast<bf16*>(q_out), qo_b, static_cast<bf16*>(key_cache), static_cast<bf16*>(value_cache),

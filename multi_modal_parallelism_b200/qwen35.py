@@ -1,12 +1,15 @@
-"""The Gated DeltaNet hybrid block stack (Qwen3.5-A3B-like, dense SwiGLU MLP in place of the MoE): gated
-delta-rule linear-attention layers and GQA attention layers in the order `Qwen35Dims.layout` gives ("GGGA":
-three delta-rule layers, then one attention layer), each followed by an MLP.
+"""The Gated DeltaNet hybrid block stack (Qwen3.5-A3B-like): gated delta-rule linear-attention layers and GQA
+attention layers in the order `Qwen35Dims.layout` gives ("GGGA": three delta-rule layers, then one attention
+layer), each followed by an MLP: a dense SwiGLU one, or with `n_experts` a mixture of experts (top-k routed
+SwiGLU experts and, optionally, one that every token takes behind a sigmoid gate). With `rope_sections` the
+attention layers take positions with several axes (time, height, width of images and video): `ctx.positions`
+[axes, rows]; one row of positions counts for every axis.
 
 The reference has no implementation of this model family: `configs/qwen35_35b_a3b.yaml:1-22` describes it and
 `harness/synth.py:114-160` models its per-layer-type layouts, which are the layouts here:
 
 * ``tp``: every layer's heads (delta-rule key/value heads, attention query heads with the key/value heads they
-  read) and MLP columns split over all ranks; one all-reduce after each mixer and after each MLP;
+  read) and MLP columns (of every expert) split over all ranks; one all-reduce after each mixer and after each MLP;
 * ``attn_dp``: the attention layers data-parallel over sequences (the whole attention weight set on every rank;
   rank r attends for its own contiguous block of sequences and reads only their keys/values), their outputs
   all-gathered; delta-rule layers and MLPs as in ``tp``.
@@ -54,6 +57,13 @@ class Qwen35Dims:
     rope_theta: float = 1e7
     layout: str = "GGGA"
     chunk: int = 64
+    n_experts: int = 0  # routed experts in place of the dense MLP (0: dense)
+    top_k: int = 8
+    moe_intermediate: int = 512  # of every expert, the shared one included
+    shared_expert: bool = False
+    rotary_dim: int = 0  # rotated dims of an attention head (0: all)
+    rope_sections: tuple = ()  # rotated pairs of each position axis (empty: positions have one axis)
+    rope_interleaved: bool = True
 
     @property
     def qkv_rows(self) -> int:
@@ -73,6 +83,8 @@ class Qwen35Dims:
         for k in ("rms_eps", "rope_theta"):
             if k in kw:
                 kw[k] = float(kw[k])
+        if "rope_sections" in kw:
+            kw["rope_sections"] = tuple(kw["rope_sections"])
         return cls(**kw)
 
     def replace(self, **kw) -> "Qwen35Dims":
@@ -109,9 +121,20 @@ def random_stack(d: Qwen35Dims, seed: int = 0) -> list[dict[str, torch.Tensor]]:
             w["self_attn.o_proj.weight"] = nrm(H, d.n_q * hd)
         else:
             raise ValueError(f"layout {d.layout!r}: layer kinds are G (delta rule) and A (attention)")
-        w["mlp.gate_proj.weight"] = nrm(I, H)
-        w["mlp.up_proj.weight"] = nrm(I, H)
-        w["mlp.down_proj.weight"] = nrm(H, I)
+        if d.n_experts:
+            E, n = d.n_experts, d.moe_intermediate
+            w["mlp.gate.weight"] = nrm(E, H)
+            w["mlp.experts.gate_up_proj"] = nrm(E * 2 * n, H).view(E, 2 * n, H)
+            w["mlp.experts.down_proj"] = nrm(E * H, n).view(E, H, n)
+            if d.shared_expert:
+                w["mlp.shared_expert.gate_proj.weight"] = nrm(n, H)
+                w["mlp.shared_expert.up_proj.weight"] = nrm(n, H)
+                w["mlp.shared_expert.down_proj.weight"] = nrm(H, n)
+                w["mlp.shared_expert_gate.weight"] = nrm(1, H)
+        else:
+            w["mlp.gate_proj.weight"] = nrm(I, H)
+            w["mlp.up_proj.weight"] = nrm(I, H)
+            w["mlp.down_proj.weight"] = nrm(H, I)
         out.append(w)
     return out
 
@@ -149,9 +172,12 @@ def attn_shard(d: Qwen35Dims, rank: int, world: int) -> AttnShard:
 
 
 def mlp_cols(d: Qwen35Dims, rank: int, world: int) -> range:
-    if d.intermediate % world:
-        raise ValueError(f"mlp_cols: intermediate {d.intermediate} does not split over {world} ranks")
-    n = d.intermediate // world
+    """Intermediate columns of this rank: of the dense MLP, or of every expert."""
+    total = d.moe_intermediate if d.n_experts else d.intermediate
+    if total % world or (d.n_experts and total // world % 8):
+        raise ValueError(f"mlp_cols: intermediate {total} does not split over {world} ranks"
+                         + (" in multiples of 8" if d.n_experts else ""))
+    n = total // world
     return range(rank * n, (rank + 1) * n)
 
 
@@ -184,6 +210,32 @@ class _Mlp:
         return K.gemm(self.act[:T], self.w_down, out=out, addend=addend)
 
 
+class _Moe:
+    """Mixture of experts over this rank's columns of every expert: the router's product, then routing, the experts'
+    products and their weighted sum (a partial sum when the columns are split; every rank routes alike). The shared
+    expert is the last of the experts, its gate the last of the router's rows."""
+
+    def __init__(self, d: Qwen35Dims, w: dict, cols: range, device: torch.device, rows: int):
+        self.d, n, I = d, cols.stop - cols.start, d.moe_intermediate
+        sl, su = slice(cols.start, cols.stop), slice(I + cols.start, I + cols.stop)
+        router, gu, down = w["mlp.gate.weight"], w["mlp.experts.gate_up_proj"], w["mlp.experts.down_proj"]
+        gu, down = torch.cat([gu[:, sl], gu[:, su]], 1), down[:, :, sl]
+        if d.shared_expert:
+            router = torch.cat([router, w["mlp.shared_expert_gate.weight"]])
+            one = torch.cat([w["mlp.shared_expert.gate_proj.weight"][sl], w["mlp.shared_expert.up_proj.weight"][sl]])
+            gu = torch.cat([gu, one[None]])
+            down = torch.cat([down, w["mlp.shared_expert.down_proj.weight"][None, :, sl]])
+        self.w_router, self.w_gu, self.w_down = _put(router, device), _put(gu, device), _put(down, device)
+        E = self.w_down.shape[0]
+        self.logits = torch.empty(rows, _pad8(E), device=device, dtype=BF16)
+        self.ws = K.moe_workspace(rows, d.top_k + d.shared_expert, d.hidden, n, E, device)
+
+    def forward(self, y: torch.Tensor, out: torch.Tensor, addend: torch.Tensor | None = None) -> torch.Tensor:
+        logits = K.gemm(y, self.w_router, out=self.logits[:y.shape[0], :self.w_router.shape[0]])
+        return K.moe_layer(y, logits, self.w_gu, self.w_down, self.d.top_k, out=out, shared=self.d.shared_expert,
+                           addend=addend, workspace=self.ws)
+
+
 class _Layer:
     """Norm, mixer, collective, residual + norm, MLP, collective, residual."""
 
@@ -192,7 +244,8 @@ class _Layer:
         self.world = groups.world_size
         self.in_norm = _put(w["input_layernorm.weight"], device)
         self.post_norm = _put(w["post_attention_layernorm.weight"], device)
-        self.mlp = _Mlp(w, mlp_cols(d, groups.rank, self.world), device, rows)
+        cols = mlp_cols(d, groups.rank, self.world)
+        self.mlp = _Moe(d, w, cols, device, rows) if d.n_experts else _Mlp(w, cols, device, rows)
         mk = lambda: torch.empty(rows, d.hidden, device=device, dtype=BF16)  # noqa: E731
         self.xn, self.mix, self.h1, self.y, self.part, self.out = mk(), mk(), mk(), mk(), mk(), mk()
 
@@ -275,7 +328,7 @@ class GdnLayer(_Layer):
 
 def _sub_decode_ctx(ctx: DecodeCtx, rows: range, cu_q: torch.Tensor) -> DecodeCtx:
     sl = slice(rows.start, rows.stop)
-    return DecodeCtx(B=len(rows), c=ctx.c, kv_block=ctx.kv_block, nblk=ctx.nblk, positions=ctx.positions[sl],
+    return DecodeCtx(B=len(rows), c=ctx.c, kv_block=ctx.kv_block, nblk=ctx.nblk, positions=ctx.positions[..., sl],
                      cu_q=cu_q, seqused_k=ctx.seqused_k[sl], block_table=ctx.block_table[sl],
                      slot_mapping=ctx.slot_mapping[sl], state_idx=ctx.state_idx[sl], max_k=ctx.max_k)
 
@@ -290,7 +343,7 @@ def _sub_prefill_ctx(ctx: PrefillCtx, seqs: range) -> tuple[PrefillCtx, range]:
     sub_cu = torch.tensor([c - r0 for c in cu[seqs.start:seqs.stop + 1]], dtype=torch.int32).to(ctx.cu_seqlens.device)
     ss, rs = slice(seqs.start, seqs.stop), slice(r0, r1)
     return PrefillCtx(nseq=len(seqs), T=r1 - r0, kv_block=ctx.kv_block, nblk=ctx.nblk, lens=lens,
-                      starts=ctx.starts[ss], cu_seqlens=sub_cu, positions=ctx.positions[rs],
+                      starts=ctx.starts[ss], cu_seqlens=sub_cu, positions=ctx.positions[..., rs],
                       slot_mapping=ctx.slot_mapping[rs], block_table=ctx.block_table[ss], ctx_start=ctx.ctx_start[ss],
                       state_idx=ctx.state_idx[ss], has_init=ctx.has_init[ss], max_len=max(lens, default=0)), range(r0, r1)
 
@@ -312,7 +365,13 @@ class AttnLayer(_Layer):
         self.wqkv = _put(torch.cat([w["self_attn.q_proj.weight"][qs], w["self_attn.k_proj.weight"][ks],
                                     w["self_attn.v_proj.weight"][ks]]), device)
         self.wo = _put(w["self_attn.o_proj.weight"][:, qs], device)
-        self.inv_freq = K.rope_inv_freq(hd, d.rope_theta, device)
+        rd = d.rotary_dim or hd
+        self.inv_freq = K.rope_inv_freq(rd, d.rope_theta, device)
+        sections = tuple(d.rope_sections) or ((rd // 2,) if rd < hd else ())
+        if sections and sum(sections) != rd // 2:
+            raise ValueError(f"AttnLayer: rope_sections {sections} do not sum to the {rd // 2} rotated pairs")
+        self.axes = K.rope_axes(sections, d.rope_interleaved, device) if sections else None
+        self.n_axes = len(sections)
         self.kv, self.key_cache, self.value_cache, _ = alloc_kv(num_blocks, kv_block, self.nkv, hd, device)
         self.qkv = torch.empty(rows, self.wqkv.shape[0], device=device, dtype=BF16)
         self.q = torch.empty(rows, self.nq * hd, device=device, dtype=BF16)
@@ -325,8 +384,15 @@ class AttnLayer(_Layer):
         """This rank's heads for the rows of x ([n, H], the rows of ctx): the o-projection into out [n, H]."""
         n, hd = x.shape[0], self.d.head_dim
         qkv = K.gemm(x, self.wqkv, out=self.qkv[:n])
-        K.qkv_rope_kv_write(qkv, self.nq, self.nkv, hd, ctx.positions, self.inv_freq, 1.0, self.q[:n], self.key_cache,
-                            self.value_cache, ctx.slot_mapping)
+        if self.axes is None:
+            K.qkv_rope_kv_write(qkv, self.nq, self.nkv, hd, ctx.positions, self.inv_freq, 1.0, self.q[:n], self.key_cache,
+                                self.value_cache, ctx.slot_mapping)
+        else:
+            pos = ctx.positions if ctx.positions.dim() == 2 else ctx.positions[None].expand(self.n_axes, -1)
+            if pos.shape[0] != self.n_axes:
+                raise ValueError(f"AttnLayer: positions {tuple(pos.shape)} for {self.n_axes} rotary axes")
+            K.qkv_mrope_kv_write(qkv, self.nq, self.nkv, hd, pos, self.inv_freq, self.axes, 1.0, self.q[:n], self.key_cache,
+                                 self.value_cache, ctx.slot_mapping)
         q, ao = self.q[:n].unflatten(1, (self.nq, hd)), self.ao[:n].unflatten(1, (self.nq, hd))
         if isinstance(ctx, PrefillCtx):
             K.attn_prefill(q, self.key_cache, self.value_cache, ctx.block_table, ctx.cu_seqlens, ctx.ctx_start,

@@ -33,7 +33,7 @@ class DecodeCtx:
     c: int
     kv_block: int
     nblk: int
-    positions: torch.Tensor  # [B] int64, position of the new token (= context length c)
+    positions: torch.Tensor  # [B] int64, position of the new token (= context length c); or [axes, B] rotary positions
     cu_q: torch.Tensor  # [B+1] int32
     seqused_k: torch.Tensor  # [B] int32, keys per sequence after this step (= c+1)
     block_table: torch.Tensor  # [B, nblk] int32
@@ -60,7 +60,7 @@ class PrefillCtx:
     lens: list[int]
     starts: list[int]
     cu_seqlens: torch.Tensor  # [nseq+1] int32
-    positions: torch.Tensor  # [T] int64, ctx_start[i] + j
+    positions: torch.Tensor  # [T] int64, ctx_start[i] + j; or [axes, T] rotary positions
     slot_mapping: torch.Tensor  # [T] int64, cache slot of every new token
     block_table: torch.Tensor  # [nseq, nblk] int32
     ctx_start: torch.Tensor  # [nseq] int32
@@ -112,11 +112,13 @@ def advance_decode_ctx(ctx: DecodeCtx, n: int = 1) -> None:
     """Move every sequence of `ctx` n tokens on, in place (positions, keys used, cache slots): the context of
     the next decode step of the same batch. The block table must already hold the new positions."""
     table = ctx.block_table
-    pos = ctx.positions + n
+    rotary = ctx.positions + n
+    # several position axes: the rotary positions are not the token's index in the cache
+    pos = rotary if rotary.dim() == 1 else ctx.seqused_k.to(torch.int64) - 1 + n
     blk = pos // ctx.kv_block
     if int(blk.max()) >= table.shape[1]:
         raise ValueError("advance_decode_ctx: block table too short for the next position")
-    ctx.positions.copy_(pos)
+    ctx.positions.copy_(rotary)
     ctx.seqused_k.add_(n)
     rows = torch.arange(ctx.B, device=table.device)
     ctx.slot_mapping.copy_(table[rows, blk].to(torch.int64) * ctx.kv_block + pos % ctx.kv_block)

@@ -36,6 +36,7 @@ from dataclasses import dataclass
 import numpy as np
 
 from .hybrid_layer import F32, conv1d_prefill, conv1d_update, gemm, rmsnorm, silu, softplus
+from .moe import moe_mlp
 
 
 def l2norm(x: np.ndarray, eps: float = 1e-6) -> np.ndarray:
@@ -153,6 +154,8 @@ def _finish(w: dict, d: GdnDims, h: np.ndarray, o: np.ndarray, z: np.ndarray) ->
     oz = oz * silu(z.reshape(T, d.n_v, d.dv))
     h1 = h + gemm(oz.reshape(T, -1), w["out_proj.weight"])
     y = rmsnorm(h1, w["post_attention_layernorm.weight"], d.rms_eps)
+    if "mlp.gate.weight" in w:  # mixture of experts
+        return h1 + moe_mlp(w, d, y)
     mlp = gemm(silu(gemm(y, w["mlp.gate_proj.weight"])) * gemm(y, w["mlp.up_proj.weight"]), w["mlp.down_proj.weight"])
     return h1 + mlp
 

@@ -262,6 +262,59 @@ def qkv_rope_kv_write(qkv, nq, nkv, head_dim, positions, inv_freq, key_mult, q_o
     return q_out
 
 
+def qkv_mrope_kv_write(qkv, nq, nkv, head_dim, positions, inv_freq, axes, key_mult, q_out, key_cache, value_cache,
+                       slot_mapping):
+    _rows16("qkv_mrope_kv_write.qkv", qkv)
+    T, half = qkv.shape[0], inv_freq.numel()
+    assert positions.shape == (int(axes.max()) + 1, T) and axes.shape == inv_freq.shape and 2 * half <= head_dim
+    ang = (positions[axes.long()].T.double() * inv_freq.double()).float()[:, None]
+    x = qkv.float().view(T, nq + 2 * nkv, head_dim)
+    qk = torch.cat([x[:, :nq], x[:, nq:nq + nkv] * key_mult], 1)
+    a, b = qk[..., :half], qk[..., half:2 * half]
+    r = torch.cat([a * ang.cos() - b * ang.sin(), b * ang.cos() + a * ang.sin(), qk[..., 2 * half:]], -1)
+    q_out.copy_(r[:, :nq].reshape(T, -1).to(q_out.dtype))
+    blk = key_cache.shape[1]
+    for t in range(T):
+        s = int(slot_mapping[t])
+        if s >= 0:
+            key_cache[s // blk, s % blk].copy_(r[t, nq:].to(key_cache.dtype))
+            value_cache[s // blk, s % blk].copy_(x[t, nq + nkv:].to(value_cache.dtype))
+    return q_out
+
+
+def rope_axes(sections, interleaved, device):
+    from multi_modal_parallelism_b200.kernels import rope_axes as real
+
+    return real(sections, interleaved, device)
+
+
+def moe_workspace(T, places, hidden, intermediate, experts, device):
+    return torch.empty(1)
+
+
+def moe_layer(x, logits, w_gate_up, w_down, top_k, out=None, renormalize=True, shared=False, addend=None, workspace=None):
+    _rows16("moe_layer.x", x)
+    E, n = w_down.shape[0] - bool(shared), w_down.shape[2]
+    assert logits.shape == (x.shape[0], E + bool(shared)) and w_gate_up.shape == (w_down.shape[0], 2 * n, x.shape[1])
+    assert workspace is not None and n % 8 == 0
+    l = logits[:, :E].float()
+    v, ids = torch.sort(l, dim=1, descending=True, stable=True)
+    w = torch.softmax(v[:, :top_k], 1) if renormalize else torch.softmax(l, 1).gather(1, ids[:, :top_k])
+    res = torch.zeros(x.shape) if addend is None else addend.float()
+
+    def expert(rows, e):
+        g, u = (rows.float() @ w_gate_up[e].float().T).chunk(2, 1)
+        return (F.silu(g) * u).to(BF16).float() @ w_down[e].float().T
+
+    for e in range(E):
+        t, k = (ids[:, :top_k] == e).nonzero(as_tuple=True)
+        res = res.index_add(0, t, w[t, k][:, None] * expert(x[t], e))
+    if shared:
+        res = res + torch.sigmoid(logits[:, E:].float()) * expert(x, E)
+    out.copy_(res.to(out.dtype))
+    return out
+
+
 def _attend(q, key_cache, value_cache, table_row, n_keys):
     """q [m, nq, hd] queries attending to keys 0 .. limit[i] (inclusive) given as n_keys [m]."""
     blk = key_cache.shape[1]

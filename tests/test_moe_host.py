@@ -108,6 +108,10 @@ def test_workspace_size_grows_with_the_request():
     size = lambda *a: _lib.lib().mmp_moe_workspace_size(*a)  # noqa: E731
     assert size(0, 2, 64, 32, 8) == 0
     assert 0 < size(4, 2, 64, 32, 8) <= size(5, 2, 64, 32, 8)
+    # scratch of a larger request serves a smaller one, whichever kernels take either
+    for rest in ((2, 64, 32, 8), (8, 2048, 512, 257), (1, 8, 8, 3), (32, 8, 8, 1024), (2, 4096, 7168, 8)):
+        got = [size(T, *rest) for T in range(1, 2200)]
+        assert all(x <= y for x, y in zip(got, got[1:])), rest
     R = 1000 * 2  # a large request holds the fp32 results and the bf16 intermediate rows
     assert size(1000, 2, 64, 32, 8) >= R * (64 * 4 + 32 * 2)
     # 64-bit sizes: 2^25 places of 8192 columns
