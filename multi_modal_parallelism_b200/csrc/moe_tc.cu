@@ -42,16 +42,40 @@ __device__ __forceinline__ void pair_load_2d(uint32_t dst, const CUtensorMap* ma
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];\n"
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y) : "memory");
 }
-__device__ __forceinline__ void pair_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5}], [%2];\n"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+// Weights: ONCE where most experts have one row block, so that they are the first to leave L2 (777 tokens x 4 of 60 experts
+// 199 -> 193 us; with several blocks an expert they are read again: 2 of 8 large experts 1164 -> 1227 us).
+__device__ __forceinline__ uint64_t evict_first_policy() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;\n" : "=l"(p));
+  return p;
 }
-__device__ __forceinline__ void pair_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int u, int v) {
+template <bool ONCE>
+__device__ __forceinline__ void pair_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, uint64_t policy) {
+  if constexpr (!ONCE) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5}], [%2];\n"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+    return;
+  }
   asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5, %6, %7}], "
-      "[%2];\n"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(u), "r"(v) : "memory");
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2.L2::cache_hint [%0], "
+      "[%1, {%3, %4, %5}], [%2], %6;\n"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "l"(policy) : "memory");
+}
+template <bool ONCE>
+__device__ __forceinline__ void pair_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int u, int v,
+                                             uint64_t policy) {
+  if constexpr (!ONCE) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], "
+        "[%1, {%3, %4, %5, %6, %7}], [%2];\n"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(u), "r"(v) : "memory");
+    return;
+  }
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2.L2::cache_hint [%0], "
+      "[%1, {%3, %4, %5, %6, %7}], [%2], %8;\n"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(u), "r"(v), "l"(policy) : "memory");
 }
 __device__ __forceinline__ void pair_mma(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -90,6 +114,8 @@ template <bool UP, int STAGES, int ROWS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
     moe_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const MoeArgs A, int tiles) {
   using L = MLayout<STAGES, ROWS>;
+  constexpr bool ONCE = ROWS == MOE_BLOCK_ROWS_FEW;
+  constexpr int BOX = 64;  // rows of a TMA box of B
   extern __shared__ uint8_t dsmem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_addr(smem);
@@ -137,6 +163,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
 
   int issued = 0;  // stages requested by warp 0 (drained at teardown after an abort)
   if (warp == 0) {
+    const uint64_t policy = evict_first_policy();
     int kc = 0, early = 0;
     bool ok = true;
     if (pair < nitems) {
@@ -146,8 +173,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
       if (lane == 0)
         for (int kt = 0; kt < early; ++kt) {
           const uint32_t a_s = sbase + kt * L::STAGE_BYTES, bar = mapa(full_bar(kt), 0);
-          if (UP) pair_load_5d(a_s, &tmA, bar, kt * MK, 0, 0, tile * 8, blk.expert);
-          else pair_load_3d(a_s, &tmA, bar, kt * MK, tile * 128, blk.expert);
+          if (UP) pair_load_5d<ONCE>(a_s, &tmA, bar, kt * MK, 0, 0, tile * 8, blk.expert, policy);
+          else pair_load_3d<ONCE>(a_s, &tmA, bar, kt * MK, tile * 128, blk.expert, policy);
         }
     }
     __syncwarp();
@@ -159,8 +186,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
       // this block's half of the MMA's N rows, in boxes of 64 (what lies past it is not read; boxes of 32 or 16
       // copy less and cost 6 and 20 % more where the MMAs bound the kernel: each box is an instruction)
       const int half = (blk.n + 15) / 16 * 8;
-      const int nb = (half + 63) / 64;
-      const uint32_t bytes = 2 * (L::A_BYTES + nb * 64 * (MK * 2));
+      const int nb = (half + BOX - 1) / BOX;
+      const uint32_t bytes = 2 * (L::A_BYTES + nb * BOX * (MK * 2));
       for (int kt = 0; kt < k_tiles; ++kt, ++kc) {
         const int s = kc % STAGES;
         if (kc >= STAGES) {
@@ -173,11 +200,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
         if (lane == 0) {
           if (rank == 0) mbar_expect_tx(full_bar(s), bytes);
           if (kc >= early) {
-            if (UP) pair_load_5d(a_s, &tmA, bar, kt * MK, 0, 0, tile * 8, blk.expert);
-            else pair_load_3d(a_s, &tmA, bar, kt * MK, tile * 128, blk.expert);
+            if (UP) pair_load_5d<ONCE>(a_s, &tmA, bar, kt * MK, 0, 0, tile * 8, blk.expert, policy);
+            else pair_load_3d<ONCE>(a_s, &tmA, bar, kt * MK, tile * 128, blk.expert, policy);
           }
         }
-        if (lane < nb) pair_load_2d(b_s + lane * 64 * MK * 2, &tmB, bar, kt * MK, blk.row0 + static_cast<int>(rank) * half + lane * 64);
+        if (lane < nb) pair_load_2d(b_s + lane * BOX * MK * 2, &tmB, bar, kt * MK, blk.row0 + static_cast<int>(rank) * half + lane * BOX);
         ++issued;
       }
     }
