@@ -144,7 +144,7 @@ int mmp_rope_kv_write(const void* q, int64_t q_b, const void* k, int64_t k_b, co
  * inv_freq, axes: [rd / 2] fp32 / int32 (an axis outside [0, naxes) sets
  * MMP_DEVERR_INDEX and counts as axis 0). q goes to q_out [T, nq hd] (row stride qo_b; may be the q part of qkv itself);
  * key_mult * k, rotated, and v go to the caches at slot_mapping[t] (neither where it is < 0; a slot past the cache sets
- * MMP_DEVERR_INDEX); caches as in mmp_rope_kv_write. Any hd <= 1024 and even rd <= hd; 16-byte accesses where rd / 2, hd and
+ * MMP_DEVERR_INDEX); caches as in mmp_rope_kv_write. Any hd <= 1024, nq <= 1024, nkv <= 512 and even rd <= hd; 16-byte accesses where rd / 2, hd and
  * the rows are multiples of 8 values, single values otherwise. Slots must differ.
  */
 int mmp_mrope_kv_write(const void* qkv, int64_t row, int nq, int nkv, int hd, const int64_t* positions, int64_t p_a,
