@@ -64,7 +64,7 @@ def _device(name: str, *ts: torch.Tensor | None) -> int:
     return d
 
 
-def _call_on(d: int, name: str, *args, kernels: int = 1) -> None:
+def _call_on(d: int, name: str, args: tuple, kernels: int = 1) -> None:
     """_lib.call with device d as the current one (the library launches on the current device)."""
     if d < 0 or d == torch._C._cuda_getDevice():
         _lib.call(name, *args, kernels=kernels)
@@ -304,11 +304,11 @@ def qkv_mrope_kv_write(qkv: torch.Tensor, nq: int, nkv: int, head_dim: int, posi
         raise ValueError(f"{name}: positions and slot_mapping must be int64, inv_freq fp32 and axes int32")
     T, row = _rows(name, "qkv", qkv, (nq + 2 * nkv) * head_dim)
     Tq, qo_b = _rows(name, "q_out", q_out, nq * head_dim)
-    ps = positions.shape
-    if len(ps) != 2 or ps[1] != T or Tq != T or (T > 1 and positions.stride(1) != 1):
+    ps, pt = positions.shape, positions.stride()
+    if len(ps) != 2 or ps[1] != T or Tq != T or (T > 1 and pt[1] != 1):
         raise ValueError(f"{name}: positions must be [axes, {T}] with contiguous rows, got {tuple(ps)}; q_out has {Tq} rows")
-    half = inv_freq.shape[0] if inv_freq.dim() == 1 else 0
-    if axes.shape != inv_freq.shape or not inv_freq.is_contiguous() or not axes.is_contiguous():
+    half = inv_freq.shape
+    if len(half) != 1 or axes.shape != half or not (inv_freq.is_contiguous() and axes.is_contiguous()):
         raise ValueError(f"{name}: inv_freq and axes must be contiguous vectors of one length")
     if slot_mapping.shape != (T,) or not slot_mapping.is_contiguous():
         raise ValueError(f"{name}: slot_mapping must be a contiguous [{T}]")
@@ -317,9 +317,10 @@ def qkv_mrope_kv_write(qkv: torch.Tensor, nq: int, nkv: int, head_dim: int, posi
         raise ValueError(f"{name}: key/value caches must be [blocks, block, {nkv}, {head_dim}] views with equal strides, got "
                          f"{tuple(cs)} and {tuple(value_cache.shape)}")
     err, stream = _err_and_stream(d, qkv)
-    _call_on(d, "mmp_mrope_kv_write", qkv.data_ptr(), row, nq, nkv, head_dim, positions.data_ptr(), positions.stride(0), ps[0],
-             inv_freq.data_ptr(), axes.data_ptr(), 2 * half, key_mult, q_out.data_ptr(), qo_b, key_cache.data_ptr(),
-             value_cache.data_ptr(), st[0], st[1], st[2], cs[1], cs[0], slot_mapping.data_ptr(), T, err, stream)
+    _call_on(d, "mmp_mrope_kv_write", (qkv.data_ptr(), row, nq, nkv, head_dim, positions.data_ptr(), pt[0], ps[0],
+                                       inv_freq.data_ptr(), axes.data_ptr(), 2 * half[0], key_mult, q_out.data_ptr(), qo_b,
+                                       key_cache.data_ptr(), value_cache.data_ptr(), st[0], st[1], st[2], cs[1], cs[0],
+                                       slot_mapping.data_ptr(), T, err, stream))
     return q_out
 
 
@@ -754,8 +755,8 @@ def moe_route(logits: torch.Tensor, top_k: int, weights: torch.Tensor | None = N
     dt = _LOGITS.get(logits.dtype)
     if dt is None or logits.dim() != 2:
         raise ValueError(f"{name}: logits must be [T, experts] in fp32 or bf16, got {tuple(logits.shape)} {logits.dtype}")
-    sh = 1 if shared else 0
-    T, l_t = _rows(name, "logits", logits, logits.shape[1])
+    sh, n = 1 if shared else 0, logits.shape[1]
+    T, l_t = _rows(name, "logits", logits, n)
     shape = (T, top_k + sh)
     if weights is None:
         weights = torch.empty(shape, dtype=torch.float32, device=logits.device)
@@ -765,8 +766,8 @@ def moe_route(logits: torch.Tensor, top_k: int, weights: torch.Tensor | None = N
         ids = torch.empty(shape, dtype=torch.int32, device=logits.device)
     elif ids.dtype != torch.int32 or ids.shape != shape or not ids.is_contiguous():
         raise ValueError(f"{name}: ids must be a contiguous int32 {shape}, got {tuple(ids.shape)} {ids.dtype}")
-    _call_on(d, "mmp_moe_route", logits.data_ptr(), dt, l_t, T, logits.shape[1] - sh, top_k, 1 if renormalize else 0, sh,
-             weights.data_ptr(), ids.data_ptr(), _stream(logits))
+    _call_on(d, "mmp_moe_route", (logits.data_ptr(), dt, l_t, T, n - sh, top_k, 1 if renormalize else 0, sh, weights.data_ptr(),
+                                  ids.data_ptr(), _stream(logits)))
     return weights, ids
 
 
@@ -835,8 +836,8 @@ def moe_experts(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, 
         raise ValueError(f"{name}: weights {tuple(weights.shape)} and ids {tuple(ids.shape)} differ")
     T, H, I, E, x_t, w, io, out, ws, n = _moe_args(name, x, w_gate_up, w_down, addend, out, workspace, places)
     err, stream = _err_and_stream(d, x)
-    _call_on(d, "mmp_moe_experts", x.data_ptr(), x_t, *w, weights.data_ptr(), w_t, ids.data_ptr(), id_t, *io, T, places, H, I, E,
-             ws.data_ptr(), n, err, stream, kernels=_moe_launches(T, places, H, I, E, False))
+    _call_on(d, "mmp_moe_experts", (x.data_ptr(), x_t, *w, weights.data_ptr(), w_t, ids.data_ptr(), id_t, *io, T, places, H, I, E,
+                                    ws.data_ptr(), n, err, stream), _moe_launches(T, places, H, I, E, False))
     return out
 
 
@@ -858,6 +859,6 @@ def moe_layer(x: torch.Tensor, logits: torch.Tensor, w_gate_up: torch.Tensor, w_
     if Tl != T:
         raise ValueError(f"{name}: logits {tuple(logits.shape)} is not [{T}, {E}]")
     err, stream = _err_and_stream(d, x)
-    _call_on(d, "mmp_moe_layer", x.data_ptr(), x_t, logits.data_ptr(), dt, l_t, *w, *io, T, top_k, 1 if renormalize else 0, sh, H, I,
-             E, ws.data_ptr(), n, err, stream, kernels=_moe_launches(T, places, H, I, E, True))
+    _call_on(d, "mmp_moe_layer", (x.data_ptr(), x_t, logits.data_ptr(), dt, l_t, *w, *io, T, top_k, 1 if renormalize else 0, sh, H, I,
+                                  E, ws.data_ptr(), n, err, stream), _moe_launches(T, places, H, I, E, True))
     return out
