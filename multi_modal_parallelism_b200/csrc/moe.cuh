@@ -32,13 +32,16 @@ struct MoeGroup {
 };
 
 // The few-token kernels where experts have few rows, the tensor-core kernels else. Measured (us, few-token / tensor-core):
-// 576 places on 257 experts of 6.3 MB 222 / 225, 1152 places 327 / 268; 32 on 8 of 176 MB 299 / 254; 256 on 60 of 17 MB
-// 205 / 174. Where the experts together are small the latter's five launches weigh more: 64 places on 8 of 6.3 MB 20 / 32,
-// 256 on 60 of 3.1 MB 47 / 55, 512 on 16 of 1.6 MB 29 / 26.
+// 576 places on 257 experts of 6.3 MB 212 / 218, 900 places 251 / 248, 1152 places 327 / 261; 256 on 60 of 17 MB 190 / 169. The
+// down product has a block for 16 columns of H: with few of them it does not fill the GPU (160 places on 128 of 12.6 MB, H 1024:
+// 229 / 186). Where the experts together are small the latter's five launches weigh more: 64 places on 8 of 6.3 MB 18 / 30,
+// 256 on 60 of 3.1 MB 45 / 54, 512 on 16 of 1.6 MB 29 / 26.
+inline bool moe_is_tiny(int64_t T, int places) { return T <= MOE_TINY_TOKENS && T * places <= MOE_TINY_PLACES; }
 inline bool moe_is_few(int64_t T, int places, int H, int I, int E) {
   const int64_t R = T * places;
+  if (moe_is_tiny(T, places)) return true;
   if (R > MOE_FEW_PLACES) return false;
-  return 2 * R <= 5 * E || (R <= 12 * E && 6LL * E * H * I <= 200000000);
+  return (2 * R <= 5 * E && H >= 1536) || (R <= 12 * E && 6LL * E * H * I <= 200000000);
 }
 
 // Workspace offsets in bytes, every part 256-byte aligned.
@@ -104,9 +107,8 @@ struct RouteParams {
 // group.
 struct MoeFewPlan { bool tiny; int rows; };
 inline MoeFewPlan moe_few_plan(const MoeArgs& A) {
-  const int R = A.T * A.places;
-  const bool tiny = A.T <= MOE_TINY_TOKENS && R <= MOE_TINY_PLACES;
-  return {tiny, tiny || R <= 4 * A.E ? 8 : 16};
+  const bool tiny = moe_is_tiny(A.T, A.places);
+  return {tiny, tiny || A.T * A.places <= 4 * A.E ? 8 : 16};
 }
 // The few-token products (moe_few.cu) and the sum into A.out.
 int moe_products_few(const MoeArgs& A, const RouteParams& P, bool f32, const MoeFewPlan& plan, cudaStream_t s);
