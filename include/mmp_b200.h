@@ -140,12 +140,11 @@ int mmp_rope_kv_write(const void* q, int64_t q_b, const void* k, int64_t k_b, co
  * images and video carry a position for each axis (time, height, width). qkv: [T, (nq + 2 nkv) hd] bf16 rows [q | k | v]
  * with row stride `row`. Pair i < rd / 2 of a head (dims i and i + rd / 2; dims >= rd are not rotated) of q and of
  * key_mult * k turns by positions[axes[i], t] * inv_freq[i], the product taken exactly (far positions keep their angle).
- * positions: [naxes, T] int64, rows of stride p_a (0: one row for all axes);
- * inv_freq, axes: [rd / 2] fp32 / int32 (an axis outside [0, naxes) sets
- * MMP_DEVERR_INDEX and counts as axis 0). q goes to q_out [T, nq hd] (row stride qo_b; may be the q part of qkv itself);
+ * positions: [naxes, T] int64, rows of stride p_a (0: one row for all axes); inv_freq, axes: [rd / 2] fp32 / int32 (an axis
+ * outside [0, naxes) sets MMP_DEVERR_INDEX and counts as axis 0). q goes to q_out [T, nq hd] (row stride qo_b; may be the q part of qkv itself);
  * key_mult * k, rotated, and v go to the caches at slot_mapping[t] (neither where it is < 0; a slot past the cache sets
- * MMP_DEVERR_INDEX); caches as in mmp_rope_kv_write. Any hd <= 1024, nq <= 1024, nkv <= 512 and even rd <= hd; 16-byte accesses where rd / 2, hd and
- * the rows are multiples of 8 values, single values otherwise. Slots must differ.
+ * MMP_DEVERR_INDEX); caches as in mmp_rope_kv_write. Any hd <= 1024, nq <= 1024,
+ * nkv <= 512 and even rd <= hd; 16-byte accesses where rd / 2, hd and the rows are multiples of 8 values, single values else. Slots must differ.
  */
 int mmp_mrope_kv_write(const void* qkv, int64_t row, int nq, int nkv, int hd, const int64_t* positions, int64_t p_a,
                        int naxes, const float* inv_freq, const int32_t* axes, int rd, float key_mult, void* q_out,
@@ -393,8 +392,9 @@ int mmp_gdn_prefill_tc(const void* q, int64_t q_t, int64_t q_h, const void* k, i
  * mmp_moe_workspace_size(T, places, H, I, E) bytes, scratch of this call alone: calls that may overlap on the GPU, captured
  * ones among them, need one each.
  *
- * mmp_moe_layer: both from the logits ([T, E], columns as mmp_moe_route takes them); with at most 8 tokens (and
- * 64 places) routing, both products and the sum are one cooperative launch. E counts the experts of the weight tensors, the shared one (their last) included. */
+ * mmp_moe_layer: both from the logits ([T, E], columns as mmp_moe_route takes them); with at most 8 tokens (and 64 places)
+ * routing, both products and the sum are one cooperative launch. E counts the experts of the weight tensors, the shared one
+ * (their last) included. */
 int mmp_moe_route(const void* logits, int logits_dtype, int64_t l_t, int T, int E, int top_k, int renormalize, int shared,
                   float* weights, int32_t* ids, void* stream);
 size_t mmp_moe_workspace_size(int T, int places, int H, int I, int E);

@@ -50,6 +50,13 @@ struct MoeLayout {
   int max_blocks;
 };
 
+// L2 policy of data that is read once: the first to leave.
+__device__ __forceinline__ uint64_t evict_first_policy() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;\n" : "=l"(p));
+  return p;
+}
+
 inline size_t moe_align(size_t n) { return (n + 255) / 256 * 256; }
 
 inline MoeLayout moe_layout(int64_t T, int places, int H, int I, int E) {

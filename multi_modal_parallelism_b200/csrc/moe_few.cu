@@ -31,11 +31,6 @@ __device__ __forceinline__ void mma_16816(float* c, uint32_t a0, uint32_t a1, ui
 }
 // 16 bytes to shared memory, zeros where !valid. Weights are the first to leave L2 (64 tokens x 8 of 256 experts 222 -> 215 us:
 // what the next kernels read stays).
-__device__ __forceinline__ uint64_t evict_first_policy() {
-  uint64_t p;
-  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;\n" : "=l"(p));
-  return p;
-}
 __device__ __forceinline__ void copy_weight(uint32_t dst, const bf16* p, bool valid, uint64_t policy) {
   asm volatile("cp.async.cg.shared.global.L2::cache_hint.L2::128B [%0], [%1], 16, %2, %3;\n"
                ::"r"(dst), "l"(p), "r"(valid ? 16 : 0), "l"(policy) : "memory");
@@ -339,9 +334,10 @@ __device__ __forceinline__ int down_turn(int ngroups, int tile, int tiles) {
   return static_cast<int>(static_cast<int64_t>(ngroups) * tile / tiles);
 }
 
-// Output columns r0 .. r0 + 16 MT - 1: the warps' tasks (group, k range) into val [split][place][16 MT]. Blocks start at different groups (`turn`), so
-// that they do not all read the same rows of h at once. ready() is called by every warp
-// once its first weights are requested, and returns when h is written.
+// Output columns r0 .. r0 + 16 MT - 1: the warps' tasks (group, k range) into val [split][place][16 MT]. Blocks start at
+// different groups (`turn`), so that they do not all read the same rows of h at once (32 tokens x 4 of 60 experts, I 1408: the
+// kernel took 73 us instead of 64). ready() is called by every warp once its first weights are requested, and returns when
+// h is written.
 template <int MT, int NF, int D, typename G, typename Ready>
 __device__ __forceinline__ void down_tasks(const MoeArgs& A, const G* groups, int ngroups, int splits, int r0, int warp, int warps,
                                            int lane, int turn, Queue<MT, NF, D>& q, float* val, Ready ready) {
@@ -519,7 +515,7 @@ __global__ void __launch_bounds__(WARPS * 32) moe_down_few(const MoeArgs A, int 
 // ------------------------------------------------------------------------------------------------ tiny: one kernel
 // At most 8 tokens and 64 places: the whole layer in one cooperative launch of a block an SM. Every block plans (and routes)
 // for itself; four crews of 8 warps take up units; then every warp requests its first down weights and the grid meets; then
-// all 32 warps take down tasks. 1 token x 9 of 257 experts (H 2048, I 512): as two launches 24.7 us.
+// all 32 warps take down tasks. 1 token x 9 of 257 experts (H 2048, I 512): 21.4 us, as two launches 24.7.
 constexpr int TINY_WARPS = 32, TINY_D = 2, TINY_RED = TINY_WARPS * 512;
 constexpr int TINY_SHARED = TINY_WARPS * Queue<1, 1, TINY_D>::BYTES + TINY_RED + static_cast<int>(sizeof(TinyPlan));
 
@@ -533,8 +529,8 @@ __global__ void __launch_bounds__(TINY_WARPS * 32, 1) moe_tiny(const MoeArgs A, 
   q.base = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * Queue<1, 1, TINY_D>::BYTES + lane * 16;
   tiny_plan<V, F32>(A, P, S, blockIdx.x == 0);
   up_units(A, S.g, S.ngroups, blockIdx.x + gridDim.x * crew, gridDim.x * (TINY_WARPS / UP_WARPS), warp % UP_WARPS, lane, q,
-                      reinterpret_cast<float4*>(red + crew * UP_WARPS * 512),
-                      [=]() { asm volatile("bar.sync %0, %1;\n" ::"r"(crew + 1), "n"(UP_WARPS * 32) : "memory"); });
+           reinterpret_cast<float4*>(red + crew * UP_WARPS * 512),
+           [=]() { asm volatile("bar.sync %0, %1;\n" ::"r"(crew + 1), "n"(UP_WARPS * 32) : "memory"); });
   const int R = A.T * A.places, tiles = (A.H + 15) / 16;
   const int splits = down_splits(S.ngroups, (A.I + STEP - 1) / STEP, TINY_WARPS, TINY_RED / (R * 64), lane);
   float* val = reinterpret_cast<float*>(red);

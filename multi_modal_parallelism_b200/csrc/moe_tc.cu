@@ -44,11 +44,6 @@ __device__ __forceinline__ void pair_load_2d(uint32_t dst, const CUtensorMap* ma
 }
 // Weights: ONCE where most experts have one row block, so that they are the first to leave L2 (777 tokens x 4 of 60 experts
 // 199 -> 193 us; with several blocks an expert they are read again: 2 of 8 large experts 1164 -> 1227 us).
-__device__ __forceinline__ uint64_t evict_first_policy() {
-  uint64_t p;
-  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;\n" : "=l"(p));
-  return p;
-}
 template <bool ONCE>
 __device__ __forceinline__ void pair_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, uint64_t policy) {
   if constexpr (!ONCE) {

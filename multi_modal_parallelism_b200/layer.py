@@ -47,6 +47,8 @@ class AttentionBranch:
         (the fused projections of a rank that holds both)."""
         a = plan.attn
         assert a is not None
+        if ctx.positions.dim() != 1:
+            raise ValueError(f"AttentionBranch: positions {tuple(ctx.positions.shape)} for a rotation with one axis")
         self.plan, self.w, self.dims, self.st, self.ctx = plan, w, dims, st, ctx
         self.nq, self.nkv, self.hd = len(a.q_heads), len(a.kv_heads), dims.head_dim
         self.inv_freq = K.rope_inv_freq(self.hd, dims.rope_theta, device)

@@ -385,6 +385,8 @@ class AttnLayer(_Layer):
         n, hd = x.shape[0], self.d.head_dim
         qkv = K.gemm(x, self.wqkv, out=self.qkv[:n])
         if self.axes is None:
+            if ctx.positions.dim() != 1:
+                raise ValueError(f"AttnLayer: positions {tuple(ctx.positions.shape)} for a rotation with one axis")
             K.qkv_rope_kv_write(qkv, self.nq, self.nkv, hd, ctx.positions, self.inv_freq, 1.0, self.q[:n], self.key_cache,
                                 self.value_cache, ctx.slot_mapping)
         else:

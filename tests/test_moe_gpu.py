@@ -312,3 +312,76 @@ def test_two_streams_at_once(T):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(o, want[i]) for o in got[i])
+
+
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("T", [5, 40, 700])
+def test_layer_rows_whose_mask_leaves_nothing(T, renorm):
+    """A token with every expert masked gets the addend alone, with the shared expert that one's share."""
+    E, k, H, I = 16, 4, 256, 64
+    x, wgu, wd, _, _, add = make(T, E + 1, 1, H, I)
+    l = torch.randn(T, E + 1, device=DEV, generator=gen(4)).to(BF)
+    l[[1, T - 1], :E] = -INF
+    out = K.moe_layer(x, l[:, :E], wgu[:E], wd[:E], k, renormalize=renorm, addend=add)
+    assert torch.equal(out[[1, T - 1]], add[[1, T - 1]])
+    w, ids = K.moe_route(l[:, :E], k, renormalize=renorm)
+    assert ids[1].tolist() == [-1] * k
+    assert torch.equal(out, K.moe_experts(x, wgu[:E], wd[:E], w, ids, addend=add))
+    check_experts(out, x, wgu[:E], wd[:E], w, ids, add)
+    out = K.moe_layer(x, l, wgu, wd, k, renormalize=renorm, shared=True, addend=add)
+    w, ids = K.moe_route(l, k, renormalize=renorm, shared=True)
+    assert ids[1].tolist() == [-1] * k + [E]
+    check_experts(out, x, wgu, wd, w, ids, add)
+
+
+def test_one_scratch_for_calls_of_every_path_in_a_row():
+    """Calls that follow one another on a stream share one scratch, sized for the largest; none is waited for."""
+    E, k, H, I = 16, 4, 512, 128
+    batches = [3, 900, 40, 8, 1500, 200, 1, 64]
+    data = [make(T, E, k, H, I, seed=T) for T in batches]
+    want = [K.moe_experts(*a[:5], addend=a[5]) for a in data]
+    ws = K.moe_workspace(max(batches), k, H, I, E, DEV)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = [K.moe_experts(*a[:5], addend=a[5], workspace=ws) for a in data]
+    for g, w in zip(got, want):
+        assert torch.equal(g, w)
+
+
+@pytest.mark.parametrize("T", [8, 40, 600])
+def test_two_captured_graphs_with_a_scratch_each(T):
+    E, k, H, I = 16, 4, 256, 64
+    data = [make(T, E, k, H, I, seed=s) for s in (1, 2)]
+    want = [K.moe_experts(*a[:5], addend=a[5]) for a in data]
+    graphs, outs, streams = [], [], [torch.cuda.Stream(DEV) for _ in data]
+    for a in data:
+        ws, out = K.moe_workspace(T, k, H, I, E, DEV), torch.empty(T, H, dtype=BF, device=DEV)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(4):
+                K.moe_experts(*a[:5], addend=a[5], out=out, workspace=ws)
+        graphs.append(graph)
+        outs.append((out, ws))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for (out, _), w in zip(outs, want):
+        assert torch.equal(out, w)
+
+
+def test_chained_layers_read_what_the_one_before_wrote():
+    """Each call's output is the next one's input, on every path, without a wait: the same bits as with one."""
+    E, k, H, I = 16, 4, 256, 64
+    for T in (8, 40, 600):
+        x, wgu, wd, w, ids, _ = make(T, E, k, H, I, seed=T)
+        y = x
+        for _ in range(6):
+            y = K.moe_experts(y, wgu, wd, w, ids, addend=y)
+        z = x
+        for _ in range(6):
+            torch.cuda.synchronize()
+            z = K.moe_experts(z, wgu, wd, w, ids, addend=z)
+        assert torch.equal(y, z)

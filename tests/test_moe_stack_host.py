@@ -117,6 +117,31 @@ def test_rotary_sections_that_do_not_fill_the_rotation_are_refused():
         Q.Qwen35Stack(d, random_stack(d, 0), "tp", g, torch.device("cpu"), 2, 4, 16, 8)
 
 
+def test_positions_with_several_axes_are_refused_where_the_rotation_has_one():
+    from types import SimpleNamespace
+
+    from multi_modal_parallelism_b200 import qwen35 as Q
+    from multi_modal_parallelism_b200.dist import Coordinator, Groups
+    from multi_modal_parallelism_b200.layer import AttentionBranch
+    from multi_modal_parallelism_b200.state import make_prefill_ctx
+    from tests import _kernel_stand_ins as S
+
+    Q.K = S
+    cpu = torch.device("cpu")
+    g = Groups(rank=0, local_rank=0, world_size=1, tp=Coordinator((0,), None), pair=None, device=cpu)
+    d = DIMS.replace(rope_sections=(), rotary_dim=0, layout="A")
+    ctx = make_prefill_ctx([8], 16, cpu)
+    several = dataclasses.replace(ctx, positions=ctx.positions.expand(3, -1))
+    stack = Q.Qwen35Stack(d, random_stack(d, 0), "tp", g, cpu, 2, 4, 16, 8)
+    x = torch.zeros(8, d.hidden, dtype=torch.bfloat16)
+    stack.step(x, ctx)
+    with pytest.raises(ValueError, match="one axis"):
+        stack.step(x, several)
+    plan = SimpleNamespace(attn=SimpleNamespace(q_heads=[0], kv_heads=[0]))
+    with pytest.raises(ValueError, match="one axis"):
+        AttentionBranch(plan, None, None, None, several, cpu)
+
+
 def test_yaml_of_the_moe_stack():
     d = Qwen35Dims.from_yaml("qwen35_moe_like")
     assert (d.n_experts, d.top_k, d.moe_intermediate, d.shared_expert) == (256, 8, 512, True)
