@@ -12,8 +12,8 @@
 //   * down: A is 128 rows of Wd, B the expert's consecutive rows of h. fp32 results per place go to y, and moe_combine sums
 //     each token's places in their order.
 // One persistent block an SM, two of them a pair on 256 weight rows (cta_group::2): each loads its own weights and half of the
-// rows, so a stage of the MMAs takes 32 KB an SM instead of 48. Warp 0 streams both operands through a ring of shared-memory
-// stages across tiles, one lane of the leader's warp 1 issues the MMAs into one of two TMEM accumulators, warps 2-5 drain the
+// rows, so 64 columns of K take 32 KB an SM instead of 48. Warps 0 and 6 stream the weights and the rows through a ring of
+// shared-memory stages across tiles, the leader's warp 1 issues the MMAs into one of two TMEM accumulators, warps 2-5 drain the
 // other.
 #include <algorithm>
 
@@ -23,12 +23,14 @@
 namespace mmp {
 namespace {
 
-constexpr int MK = 64, MTHREADS = 192;
+// A stage is SUB tiles of 64 columns of K: with one, the thread that issues the MMAs waits and commits twice as often (2 of 8 large
+// experts, 4096 tokens: 1131 us instead of 1094).
+constexpr int MK = 64, SUB = 2, MTHREADS = 224;
 
 template <int STAGES, int ROWS>
 struct MLayout {
-  static constexpr int A_BYTES = 128 * MK * 2;                  // this block's 128 weight rows
-  static constexpr int B_BYTES = ROWS / 2 * MK * 2;             // its half of the rows
+  static constexpr int A_BYTES = SUB * 128 * MK * 2;                  // this block's 128 weight rows
+  static constexpr int B_BYTES = SUB * ROWS / 2 * MK * 2;             // its half of the rows
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int BARS = STAGES * STAGE_BYTES;  // full[S], empty[S], acc_full[2], acc_empty[2]
   static constexpr int TMEM_SLOT = BARS + 8 * (2 * STAGES + 4);
@@ -72,10 +74,17 @@ __device__ __forceinline__ void pair_load_5d(uint32_t dst, const CUtensorMap* ma
       "[%1, {%3, %4, %5, %6, %7}], [%2], %8;\n"
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(u), "r"(v), "l"(policy) : "memory");
 }
-__device__ __forceinline__ void pair_mma(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+// Operands by the low words of their descriptors (start address / 16), the rest of which is the same for all of them.
+__device__ __forceinline__ void pair_mma(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n"
-      ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate));
+      "{\n.reg .pred p;\n.reg .b64 a, b;\nmov.b64 a, {%1, %3};\nmov.b64 b, {%2, %3};\nsetp.ne.b32 p, %5, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %4, p;\n}\n"
+      ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate));
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok));
+  return ok != 0;
 }
 // arrives on the barrier at this offset in both blocks once the MMAs issued so far have completed
 __device__ __forceinline__ void pair_commit(uint32_t bar) {
@@ -111,6 +120,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
   using L = MLayout<STAGES, ROWS>;
   constexpr bool ONCE = ROWS == MOE_BLOCK_ROWS_FEW;
   constexpr int BOX = 64;  // rows of a TMA box of B
+  auto box_count = [](int n) { return ((n + 15) / 16 * 8 + BOX - 1) / BOX; };
   extern __shared__ uint8_t dsmem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_addr(smem);
@@ -118,7 +128,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
   uint32_t rank;
   asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(rank));
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
-  const int k_tiles = ((UP ? A.H : A.I) + MK - 1) / MK;
+  const int k_tiles = ((UP ? A.H : A.I) + SUB * MK - 1) / (SUB * MK);
   auto full_bar = [&](int s) { return sbase + L::BARS + 8 * s; };
   auto empty_bar = [&](int s) { return sbase + L::BARS + 8 * (STAGES + s); };
   auto accf_bar = [&](int b) { return sbase + L::BARS + 8 * (2 * STAGES + b); };
@@ -148,83 +158,99 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
   pair_sync();  // both blocks' barriers are set up and their TMEM is allocated
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // The plan is complete: the kernel before this one let it start only after its own wait for it. Warp 0 requests its first
-  // weights before it waits for what that kernel writes, the rows of B.
+  // The plan is complete: the kernel before this one let it start only after its own wait for it. The weights' warp reads
+  // nothing else that a kernel wrote and starts at once.
   const int nitems = __ldcg(&A.header->nblk) * tiles;
   if (warp != 0) {
     pdl_wait();
     pdl_trigger();
   }
 
-  int issued = 0;  // stages requested by warp 0 (drained at teardown after an abort)
   if (warp == 0) {
-    const uint64_t policy = evict_first_policy();
-    int kc = 0, early = 0;
-    bool ok = true;
-    if (pair < nitems) {
-      const Item blk = moe_item(A, pair, tiles);
-      const int tile = blk.tile * 2 + rank;
-      early = min(k_tiles, STAGES);
-      if (lane == 0)
-        for (int kt = 0; kt < early; ++kt) {
-          const uint32_t a_s = sbase + kt * L::STAGE_BYTES, bar = mapa(full_bar(kt), 0);
-          if (UP) pair_load_5d<ONCE>(a_s, &tmA, bar, kt * MK, 0, 0, tile * 8, blk.expert, policy);
-          else pair_load_3d<ONCE>(a_s, &tmA, bar, kt * MK, tile * 128, blk.expert, policy);
-        }
-    }
-    __syncwarp();
-    pdl_wait();
-    pdl_trigger();
-    for (int it = pair; it < nitems && ok; it += npairs) {
-      const Item blk = moe_item(A, it, tiles);
-      const int tile = blk.tile * 2 + rank;
-      // this block's half of the MMA's N rows, in boxes of 64 (what lies past it is not read; boxes of 32 or 16
-      // copy less and cost 6 and 20 % more where the MMAs bound the kernel: each box is an instruction)
-      const int half = (blk.n + 15) / 16 * 8;
-      const int nb = (half + BOX - 1) / BOX;
-      const uint32_t bytes = 2 * (L::A_BYTES + nb * BOX * (MK * 2));
-      for (int kt = 0; kt < k_tiles; ++kt, ++kc) {
-        const int s = kc % STAGES;
-        if (kc >= STAGES) {
-          ok = mbar_wait(empty_bar(s), ((kc / STAGES) - 1) & 1, abort_flag, A.err);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-        }
-        const uint32_t a_s = sbase + s * L::STAGE_BYTES, b_s = a_s + L::A_BYTES;
-        const uint32_t bar = mapa(full_bar(s), 0);  // the leader's; bytes may arrive there before they are announced
-        if (lane == 0) {
+    if (lane == 0) {
+      const uint64_t policy = evict_first_policy();
+      int kc = 0;
+      bool ok = true;
+      for (int it = pair; it < nitems && ok; it += npairs) {
+        const Item blk = moe_item(A, it, tiles);
+        const int tile = blk.tile * 2 + static_cast<int>(rank);
+        const uint32_t bytes = 2 * (128 + box_count(blk.n) * BOX) * (SUB * MK * 2);
+        for (int kt = 0; kt < k_tiles; ++kt, ++kc) {
+          const int s = kc % STAGES;
+          if (kc >= STAGES && !mbar_wait(empty_bar(s), ((kc / STAGES) - 1) & 1, abort_flag, A.err)) {
+            ok = false;
+            break;
+          }
+          const uint32_t bar = mapa(full_bar(s), 0);  // the leader's; bytes may arrive there before they are announced
           if (rank == 0) mbar_expect_tx(full_bar(s), bytes);
-          if (kc >= early) {
-            if (UP) pair_load_5d<ONCE>(a_s, &tmA, bar, kt * MK, 0, 0, tile * 8, blk.expert, policy);
-            else pair_load_3d<ONCE>(a_s, &tmA, bar, kt * MK, tile * 128, blk.expert, policy);
+          for (int j = 0; j < SUB; ++j) {
+            const uint32_t a_s = sbase + s * L::STAGE_BYTES + j * 128 * MK * 2;
+            const int k = (kt * SUB + j) * MK;  // zeros past K
+            if (UP) pair_load_5d<ONCE>(a_s, &tmA, bar, k, 0, 0, tile * 8, blk.expert, policy);
+            else pair_load_3d<ONCE>(a_s, &tmA, bar, k, tile * 128, blk.expert, policy);
           }
         }
-        if (lane < nb) pair_load_2d(b_s + lane * BOX * MK * 2, &tmB, bar, kt * MK, blk.row0 + static_cast<int>(rank) * half + lane * BOX);
-        ++issued;
+      }
+    }
+    __syncwarp();
+  } else if (warp == 6) {
+    if (lane == 0) {
+      int kc = 0;
+      bool ok = true;
+      for (int it = pair; it < nitems && ok; it += npairs) {
+        const Item blk = moe_item(A, it, tiles);
+        // this block's half of the MMA's N rows, in boxes of 64 (what lies past it is not read; boxes of 32 or 16
+        // copy less and cost 6 and 20 % more where the MMAs bound the kernel: each box is an instruction)
+        const int nb = box_count(blk.n), row = blk.row0 + static_cast<int>(rank) * ((blk.n + 15) / 16 * 8);
+        for (int kt = 0; kt < k_tiles; ++kt, ++kc) {
+          const int s = kc % STAGES;
+          if (kc >= STAGES && !mbar_wait(empty_bar(s), ((kc / STAGES) - 1) & 1, abort_flag, A.err)) {
+            ok = false;
+            break;
+          }
+          const uint32_t bar = mapa(full_bar(s), 0), b_s = sbase + s * L::STAGE_BYTES + L::A_BYTES;
+          for (int j = 0; j < SUB; ++j)
+            for (int b = 0; b < nb; ++b)
+              pair_load_2d(b_s + (j * ROWS / 2 + b * BOX) * MK * 2, &tmB, bar, (kt * SUB + j) * MK, row + b * BOX);
+        }
       }
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      int kc = 0, tc = 0;
-      for (int it = pair; it < nitems && !*abort_flag; it += npairs, ++tc) {
+    // The whole warp walks through the stages and one lane issues: addresses then stay in uniform registers. In a branch of one
+    // thread the four MMAs of 64 columns took 272 clocks to issue instead of 77, and the kernel was bound by that thread
+    // (32 tokens x 2 of 8 large experts: 252 us instead of 231).
+    if (rank == 0) {
+      int s = 0, tc = 0;
+      uint32_t phase = 0;
+      const uint64_t desc = umma_desc(sbase);
+      const uint32_t lo0 = static_cast<uint32_t>(desc), hi = static_cast<uint32_t>(desc >> 32);
+      bool ok = true;
+      for (int it = pair; it < nitems && ok; it += npairs, ++tc) {
         const uint32_t idesc = umma_idesc_mn(256, (moe_item(A, it, tiles).n + 15) / 16 * 16);
         const int buf = tc & 1;
-        if (tc >= 2 && !mbar_wait(acce_bar(buf), ((tc >> 1) - 1) & 1, abort_flag, A.err)) break;
+        ok = __all_sync(0xffffffffu, tc < 2 || mbar_wait(acce_bar(buf), ((tc >> 1) - 1) & 1, abort_flag, A.err));
         tc_fence_after();
-        bool ok = true;
-        for (int kt = 0; kt < k_tiles; ++kt, ++kc) {
-          const int s = kc % STAGES;
-          if (!mbar_wait(full_bar(s), (kc / STAGES) & 1, abort_flag, A.err)) { ok = false; break; }
+        for (int kt = 0; kt < k_tiles && ok; ++kt) {
+          ok = __all_sync(0xffffffffu, mbar_try(full_bar(s), phase) || mbar_wait(full_bar(s), phase, abort_flag, A.err));
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t a_s = sbase + s * L::STAGE_BYTES, b_s = a_s + L::A_BYTES;
+          const uint32_t a_lo = lo0 + s * (L::STAGE_BYTES >> 4), b_lo = a_lo + (L::A_BYTES >> 4);
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < MK / 16; ++kk)
-            pair_mma(tmem + buf * 256, umma_desc(a_s + kk * 32), umma_desc(b_s + kk * 32), idesc, kt != 0 || kk != 0);
-          pair_commit(empty_bar(s));
+            for (int kk = 0; kk < SUB * MK / 16; ++kk)
+              pair_mma(tmem + buf * 256, a_lo + kk / 4 * (128 * MK * 2 >> 4) + kk % 4 * 2,
+                       b_lo + kk / 4 * (ROWS / 2 * MK * 2 >> 4) + kk % 4 * 2, hi, idesc, kk != 0 || kt != 0);
+            pair_commit(empty_bar(s));
+          }
+          __syncwarp();
+          if (++s == STAGES) {
+            s = 0;
+            phase ^= 1;
+          }
         }
-        if (!ok) break;
-        pair_commit(accf_bar(buf));
+        if (ok && elect_one()) pair_commit(accf_bar(buf));
+        __syncwarp();
       }
     }
     __syncwarp();
@@ -272,15 +298,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
     }
   }
 
-  // teardown: after an abort the copies of either block may still be in flight; the leader's barriers show both blocks', the
-  // other block lets the microseconds pass that they take
+  // teardown: after an abort copies may still be in flight to either block: the microseconds pass that they take
   if (tid == 0 && *abort_flag) {
-    if (rank == 0) {
-      for (int i = max(0, issued - STAGES); i < issued; ++i) mbar_drain(full_bar(i % STAGES), (i / STAGES) & 1);
-    } else {
-      const long long t0 = clock64();
-      while (clock64() - t0 < WAIT_BUDGET_CYCLES / 16) {
-      }
+    const long long t0 = clock64();
+    while (clock64() - t0 < WAIT_BUDGET_CYCLES / 16) {
     }
   }
   tc_fence_before();
@@ -358,11 +379,11 @@ int moe_products_tc(const MoeArgs& A, int max_blocks, cudaStream_t s) {
   }
   const int up = (A.I + 127) / 128, down = (A.H + 255) / 256;
   if (A.block_rows == MOE_BLOCK_ROWS_FEW) {
-    if ((rc = launch_products<true, 9, MOE_BLOCK_ROWS_FEW>(mgu, mx, A, up, max_blocks, sms, s)) != MMP_OK) return rc;
-    if ((rc = launch_products<false, 9, MOE_BLOCK_ROWS_FEW>(md, mh, A, down, max_blocks, sms, s)) != MMP_OK) return rc;
+    if ((rc = launch_products<true, 4, MOE_BLOCK_ROWS_FEW>(mgu, mx, A, up, max_blocks, sms, s)) != MMP_OK) return rc;
+    if ((rc = launch_products<false, 4, MOE_BLOCK_ROWS_FEW>(md, mh, A, down, max_blocks, sms, s)) != MMP_OK) return rc;
   } else {
-    if ((rc = launch_products<true, 6, MOE_BLOCK_ROWS>(mgu, mx, A, up, max_blocks, sms, s)) != MMP_OK) return rc;
-    if ((rc = launch_products<false, 6, MOE_BLOCK_ROWS>(md, mh, A, down, max_blocks, sms, s)) != MMP_OK) return rc;
+    if ((rc = launch_products<true, 3, MOE_BLOCK_ROWS>(mgu, mx, A, up, max_blocks, sms, s)) != MMP_OK) return rc;
+    if ((rc = launch_products<false, 3, MOE_BLOCK_ROWS>(md, mh, A, down, max_blocks, sms, s)) != MMP_OK) return rc;
   }
   return mmp_check_launch("mmp_moe_experts");
 }
