@@ -256,7 +256,9 @@ int few_products(const MoeArgs& A, const RouteParams& P, bool f32, cudaStream_t 
 }
 
 int many_products(MoeArgs& A, const MoeLayout& L, cudaStream_t s) {
-  A.block_rows = static_cast<int64_t>(A.T) * A.places <= 64 * A.E ? MOE_BLOCK_ROWS_FEW : MOE_BLOCK_ROWS;
+  // blocks of 128 rows leave room for a longer ring of weights and let them leave L2 at once (us, 128 / 256 rows a block: 60
+  // experts, I 1408, 32 rows each 170 / 187, 96 206 / 214, 192 295 / 278; 128 experts, I 768, 48 rows 221 / 231, 128 304 / 293)
+  A.block_rows = static_cast<int64_t>(A.T) * A.places <= 96 * A.E ? MOE_BLOCK_ROWS_FEW : MOE_BLOCK_ROWS;
   cudaError_t e = launch_kind(1, moe_plan_many, dim3(PLAN_BLOCKS), dim3(1024), 0, s, nullptr, 0, A);
   if (e != cudaSuccess) return mmp_set_error(MMP_ERR_CUDA, "mmp_moe_experts: %s", cudaGetErrorString(e));
   e = launch_kind(1, moe_sort_rows, dim3(A.T), dim3(256), 0, s, nullptr, 0, A);
@@ -333,7 +335,7 @@ extern "C" size_t mmp_moe_workspace_size(int T, int places, int H, int I, int E)
 
 extern "C" int mmp_moe_launches(int T, int places, int H, int I, int E, int route) {
   if (T <= 0 || places <= 0 || H <= 0 || I <= 0 || E <= 0) return 0;
-  if (!moe_is_few(T, places, H, I, E)) return 5 + (route ? 1 : 0);  // plan, sorted rows, up, down, sum; routing
+  if (!moe_is_few(T, places, H, I)) return 5 + (route ? 1 : 0);  // plan, sorted rows, up, down, sum; routing
   MoeArgs A{};
   A.T = T;
   A.places = places;
@@ -358,7 +360,7 @@ extern "C" int mmp_moe_experts(const void* x, int64_t x_t, const void* w_gate_up
     return mmp_set_error(MMP_ERR_INVALID, "mmp_moe_experts: weights and ids must be [T, places]");
   place_workspace(A, L, workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return moe_is_few(T, places, H, I, E) ? few_products(A, RouteParams{}, false, s) : many_products(A, L, s);
+  return moe_is_few(T, places, H, I) ? few_products(A, RouteParams{}, false, s) : many_products(A, L, s);
 }
 
 extern "C" int mmp_moe_layer(const void* x, int64_t x_t, const void* logits, int logits_dtype, int64_t l_t, const void* w_gate_up,
@@ -382,7 +384,7 @@ extern "C" int mmp_moe_layer(const void* x, int64_t x_t, const void* logits, int
   A.ids = ids;
   RouteParams P{logits, l_t, T, routed, top_k, renormalize ? 1 : 0, shared ? 1 : 0, w, ids};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (moe_is_few(T, places, H, I, E)) return few_products(A, P, logits_dtype == MMP_F32, s);
+  if (moe_is_few(T, places, H, I)) return few_products(A, P, logits_dtype == MMP_F32, s);
   rc = by_width<LaunchRoute>(routed, logits_dtype == MMP_F32, P, s);
   return rc != MMP_OK ? rc : many_products(A, L, s);
 }

@@ -31,17 +31,19 @@ struct MoeGroup {
   int place[16];
 };
 
-// The few-token kernels where experts have few rows, the tensor-core kernels else. Measured (us, few-token / tensor-core):
-// 576 places on 257 experts of 6.3 MB 212 / 218, 900 places 251 / 248, 1152 places 327 / 261; 256 on 60 of 17 MB 190 / 169. The
-// down product has a block for 16 columns of H: with few of them it does not fill the GPU (160 places on 128 of 12.6 MB, H 1024:
-// 229 / 186). Where the experts together are small the latter's five launches weigh more: 64 places on 8 of 6.3 MB 18 / 30,
-// 256 on 60 of 3.1 MB 45 / 54, 512 on 16 of 1.6 MB 29 / 26.
+// Which kernels take a call. Up to 8 tokens one launch; then the few-token kernels while the second product is small (R places
+// of I columns: its K dimension is I, at which the tensor-core kernels pay 128 columns and an accumulator's turn for each
+// expert), the tensor-core kernels else. Measured (us, few-token / tensor-core), H 2048 if not said:
+//   257 experts, I 64:  288 places 35 / 64, 1152 71 / 86;   I 128: 576 places 75 / 85, 1152 100 / 99
+//   60 experts,  I 256: 128 places 36 / 44, 256 46 / 48, 512 66 / 50;   I 1408: 36 places 91 / 81, 256 192 / 154
+//   16 experts,  I 448: 128 places 28 / 30, 256 35 / 31;   257 experts, I 512: 81 places 80 / 82, 288 172 / 158, 576 216 / 206
+//   8 experts,   I 2048: 18 places 46 / 46, 64 52 / 46
+// The down product of the few-token kernels has a block for 16 columns of H, with few of them it does not fill the GPU:
+//   256 experts, H 1024, I 128: 128 places 27 / 35, 256 45 / 42;   I 512: 72 places 66 / 47
 inline bool moe_is_tiny(int64_t T, int places) { return T <= MOE_TINY_TOKENS && T * places <= MOE_TINY_PLACES; }
-inline bool moe_is_few(int64_t T, int places, int H, int I, int E) {
-  const int64_t R = T * places;
-  if (moe_is_tiny(T, places)) return true;
-  if (R > MOE_FEW_PLACES) return false;
-  return (2 * R <= 5 * E && H >= 1536) || (R <= 12 * E && 6LL * E * H * I <= 200000000);
+inline bool moe_is_few(int64_t T, int places, int H, int I) {
+  const int64_t R = T * places, w = std::min(H, 2048);
+  return moe_is_tiny(T, places) || (R <= MOE_FEW_PLACES && I <= 512 && R * I <= w * w / 64);
 }
 
 // Workspace offsets in bytes, every part 256-byte aligned.
@@ -62,7 +64,7 @@ inline size_t moe_align(size_t n) { return (n + 255) / 256 * 256; }
 inline MoeLayout moe_layout(int64_t T, int places, int H, int I, int E) {
   MoeLayout L;
   const int64_t R = T * places;
-  const bool few = moe_is_few(T, places, H, I, E);
+  const bool few = moe_is_few(T, places, H, I);
   // the sum over experts of ceil(n / b) is at most R / b + E, and R
   L.max_blocks = static_cast<int>(std::min<int64_t>(R, R / MOE_BLOCK_ROWS_FEW + E));
   size_t at = 0;

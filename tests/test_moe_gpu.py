@@ -149,12 +149,13 @@ def check_experts(got, x, wgu, wd, weights, ids, addend):
     assert not bool(bad.any()), f"{int(bad.sum())} of {bad.numel()} off, worst {float((off / tol).max()):.3g} of the tolerance"
 
 
-# (tokens, experts, places, hidden, intermediate): one launch for up to 8 tokens, the few-token kernels while experts have few
-# rows, then the tensor-core ones
+# (tokens, experts, places, hidden, intermediate): one launch for up to 8 tokens, the few-token kernels while places times
+# intermediate is small, the tensor-core ones else; small sizes of either path are in both lists
 FEW = [(1, 1, 1, 8, 8), (1, 4, 1, 16, 8), (1, 8, 2, 256, 64), (2, 64, 8, 2048, 512), (5, 16, 4, 264, 72), (7, 30, 9, 2408, 136),
        (8, 8, 8, 128, 64), (9, 4, 2, 520, 40), (17, 2, 1, 128, 640), (40, 60, 4, 1000, 120), (384, 1000, 4, 64, 24),
        (30, 16, 2, 4104, 264), (300, 300, 4, 2400, 8), (33, 8, 2, 512, 136), (64, 60, 4, 104, 24), (100, 40, 3, 264, 72),
-       (20, 8, 2, 4808, 40), (1, 1024, 32, 72, 8)]
+       (20, 8, 2, 4808, 40), (1, 1024, 32, 72, 8),
+       (64, 60, 2, 2048, 512), (100, 60, 2, 2408, 136), (64, 8, 2, 2048, 264), (50, 8, 2, 4808, 40), (100, 8, 4, 2048, 72)]
 MANY = [(64, 8, 2, 4104, 264), (170, 12, 9, 96, 1032), (1537, 3, 1, 64, 24), (777, 5, 3, 8, 8), (600, 8, 4, 264, 72), (900, 16, 2, 1024, 200), (2000, 64, 8, 136, 64),
         (257, 16, 8, 2048, 512), (4097, 2, 1, 128, 328), (513, 1, 4, 72, 128), (1024, 300, 6, 64, 40)]
 
