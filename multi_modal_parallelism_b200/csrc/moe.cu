@@ -256,13 +256,13 @@ int few_products(const MoeArgs& A, const RouteParams& P, bool f32, cudaStream_t 
 }
 
 int many_products(MoeArgs& A, const MoeLayout& L, cudaStream_t s) {
-  // blocks of 128 rows leave room for a longer ring of weights and let them leave L2 at once (us, 128 / 256 rows a block: 60
-  // experts, I 1408, 32 rows each 170 / 187, 96 206 / 214, 192 295 / 278; 128 experts, I 768, 48 rows 221 / 231, 128 304 / 293)
-  A.block_rows = static_cast<int64_t>(A.T) * A.places <= 96 * A.E ? MOE_BLOCK_ROWS_FEW : MOE_BLOCK_ROWS;
+  A.block_rows = moe_block_rows(A.T, A.places, A.E);
   cudaError_t e = launch_kind(1, moe_plan_many, dim3(PLAN_BLOCKS), dim3(1024), 0, s, nullptr, 0, A);
   if (e != cudaSuccess) return mmp_set_error(MMP_ERR_CUDA, "mmp_moe_experts: %s", cudaGetErrorString(e));
-  e = launch_kind(1, moe_sort_rows, dim3(A.T), dim3(256), 0, s, nullptr, 0, A);
-  if (e != cudaSuccess) return mmp_set_error(MMP_ERR_CUDA, "mmp_moe_experts: %s", cudaGetErrorString(e));
+  if (!moe_gathers(A.block_rows)) {
+    e = launch_kind(1, moe_sort_rows, dim3(A.T), dim3(256), 0, s, nullptr, 0, A);
+    if (e != cudaSuccess) return mmp_set_error(MMP_ERR_CUDA, "mmp_moe_experts: %s", cudaGetErrorString(e));
+  }
   const int rc = moe_products_tc(A, L.max_blocks, s);
   if (rc != MMP_OK) return rc;
   e = launch_kind(1, moe_combine, dim3(A.T), dim3(256), 0, s, nullptr, 0, A);
@@ -335,7 +335,8 @@ extern "C" size_t mmp_moe_workspace_size(int T, int places, int H, int I, int E)
 
 extern "C" int mmp_moe_launches(int T, int places, int H, int I, int E, int route) {
   if (T <= 0 || places <= 0 || H <= 0 || I <= 0 || E <= 0) return 0;
-  if (!moe_is_few(T, places, H, I)) return 5 + (route ? 1 : 0);  // plan, sorted rows, up, down, sum; routing
+  if (!moe_is_few(T, places, H, I))  // plan, sorted rows, up, down, sum; routing
+    return (moe_gathers(moe_block_rows(T, places, E)) ? 4 : 5) + (route ? 1 : 0);
   MoeArgs A{};
   A.T = T;
   A.places = places;

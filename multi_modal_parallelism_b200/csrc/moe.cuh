@@ -18,6 +18,13 @@ constexpr int MOE_TINY_TOKENS = 8, MOE_TINY_PLACES = 64;  // up to which every b
 // Sorted rows of one expert that the tensor-core kernels take at a time (MMA N): 256, or 128 with a deeper ring of weights
 // where experts have few rows.
 constexpr int MOE_BLOCK_ROWS = 256, MOE_BLOCK_ROWS_FEW = 128;
+// Blocks of 128 rows leave room for a longer ring of weights and let them leave L2 at once (us, 128 / 256 rows a block: 60
+// experts, I 1408, 32 rows each 170 / 187, 96 206 / 214, 192 295 / 278; 128 experts, I 768, 48 rows 221 / 231, 128 304 / 293).
+inline int moe_block_rows(int64_t T, int places, int E) { return T * places <= 96 * E ? MOE_BLOCK_ROWS_FEW : MOE_BLOCK_ROWS; }
+// The up product's kernel of blocks of this many rows gathers them from x; else a kernel before it sorts x (us, gathered /
+// sorted: 60 experts, I 1408, 52 rows each 175 / 180; 8 of 176 MB, 8 rows 224 / 231; 256 of 6.3 MB, 64 rows 326 / 337; with 256
+// rows the gathers, 16 a block for 64 rows of K, are too many: 2 of 8 large experts, 4096 tokens 1250 / 1094).
+__host__ __device__ constexpr bool moe_gathers(int block_rows) { return block_rows == MOE_BLOCK_ROWS_FEW; }
 
 struct MoeHeader {
   int ngroups;  // groups of the few-token kernels
@@ -77,7 +84,7 @@ inline MoeLayout moe_layout(int64_t T, int places, int H, int I, int E) {
   L.pos = part(few ? 0 : R * 4);
   L.weights = part(R * 4);
   L.ids = part(R * 4);
-  L.xs = part(few ? 0 : R * H * 2);
+  L.xs = part(few || moe_gathers(moe_block_rows(T, places, E)) ? 0 : R * H * 2);
   L.h = part(R * I * 2);
   L.y = part(few ? 0 : R * H * 4);
   L.bytes = at;
@@ -100,7 +107,7 @@ struct MoeArgs {
   int4* blocks;   // {expert, its first sorted row, its rows, index among its blocks} of the row blocks
   int* rows;      // sorted row -> place
   int* pos;       // place -> sorted row, -1 where the place has no expert
-  bf16* xs;       // [sorted row][H]: x in the order of the rows (tensor-core path)
+  bf16* xs;       // [sorted row][H]: x in the order of the rows, where they are not gathered
   bf16* h;        // [sorted row][I]; few-token kernels: [place][I]
   float* y;       // [sorted row][H]
   int* err;

@@ -3,18 +3,17 @@
 //
 // The weights are the 128-row M side of the MMA and the rows of one expert (a block of at most 256, as many as there are,
 // in steps of 16) its N side: an expert's weights are read once for up to 256 tokens and little of an MMA is padding. Up to
-// about 250 rows an expert the layer is bound by reading the weights, above it by the MMAs.
+// about 250 rows an expert the layer is bound by HBM, above it by the MMAs.
 //   * up: the A tile is 64 gate and 64 up rows, alternating in groups of 8: one box of a 5-D tensor map over the
 //     [expert][gate | up][row] layout. Gate and up values of one column of h then sit 8 lanes apart in one warp. B are the
-//     expert's rows of xs, x sorted by a kernel before this one: 25 us for 4096 tokens x 8 places, where gathering from x
-//     inside this kernel cost 100 (16-byte copies by a warp for each stage: the fence that hands them to the MMA waits for
-//     all of a warp's copies) and 550 us (TMA gathers of four rows, one every 66 clocks).
+//     expert's tokens: gathered from x four rows at a time, or, where experts have many, boxes of xs, which a kernel before
+//     this one sorts (26 us for 4096 tokens x 8 places).
 //   * down: A is 128 rows of Wd, B the expert's consecutive rows of h. fp32 results per place go to y, and moe_combine sums
 //     each token's places in their order.
 // One persistent block an SM, two of them a pair on 256 weight rows (cta_group::2): each loads its own weights and half of the
-// rows, so 64 columns of K take 32 KB an SM instead of 48. Warps 0 and 6 stream the weights and the rows through a ring of
-// shared-memory stages across tiles, the leader's warp 1 issues the MMAs into one of two TMEM accumulators, warps 2-5 drain the
-// other.
+// rows, so 64 columns of K take 32 KB an SM instead of 48. Warp 0 streams the weights, warps 6 and 7 (or 6) the rows
+// through a ring of shared-memory stages across tiles, the leader's warp 1 issues the MMAs into one of two TMEM accumulators,
+// warps 2-5 drain the other.
 #include <algorithm>
 
 #include "moe.cuh"
@@ -25,7 +24,7 @@ namespace {
 
 // A stage is SUB tiles of 64 columns of K: with one, the thread that issues the MMAs waits and commits twice as often (2 of 8 large
 // experts, 4096 tokens: 1131 us instead of 1094).
-constexpr int MK = 64, SUB = 2, MTHREADS = 224;
+constexpr int MK = 64, SUB = 2, MTHREADS = 256;
 
 template <int STAGES, int ROWS>
 struct MLayout {
@@ -38,11 +37,23 @@ struct MLayout {
   static constexpr int DYN = ABORT + 4 + 1024;
 };
 
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok));
+  return ok != 0;
+}
 // TMA loads into this block's shared memory that complete on a barrier of either block of the pair (no multicast).
 __device__ __forceinline__ void pair_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];\n"
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+// four rows of a map whose box is one row high
+__device__ __forceinline__ void pair_gather4(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int4 r) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 [%0], "
+      "[%1, {%3, %4, %5, %6, %7}], [%2];\n"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w) : "memory");
 }
 // Weights: ONCE where most experts have one row block, so that they are the first to leave L2 (777 tokens x 4 of 60 experts
 // 199 -> 193 us; with several blocks an expert they are read again: 2 of 8 large experts 1164 -> 1227 us).
@@ -81,11 +92,6 @@ __device__ __forceinline__ void pair_mma(uint32_t tmem_d, uint32_t a_lo, uint32_
       "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %4, p;\n}\n"
       ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate));
 }
-__device__ __forceinline__ bool elect_one() {
-  uint32_t ok;
-  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok));
-  return ok != 0;
-}
 // arrives on the barrier at this offset in both blocks once the MMAs issued so far have completed
 __device__ __forceinline__ void pair_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"
@@ -103,9 +109,11 @@ __device__ __forceinline__ void arrive_leader(uint32_t bar) {
 // one another, so that its weights come from HBM once (2 of 8 large experts, four blocks each: block by block their 117 MB
 // would pass through L2 four times).
 struct Item { int expert, row0, n, tile; };
-__device__ __forceinline__ Item moe_item(const MoeArgs& A, int it, int tiles) {
+__device__ __forceinline__ int4 moe_block(const MoeArgs& A, int it, int tiles, int nitems) {
+  return __ldcg(A.blocks + min(it, nitems - 1) / tiles);  // past the last: not used
+}
+__device__ __forceinline__ Item moe_item(const MoeArgs& A, const int4& r, int it, int tiles) {
   const int b = it / tiles;
-  const int4 r = __ldcg(A.blocks + b);
   const int nb = (r.z + A.block_rows - 1) / A.block_rows, q = it - (b - r.w) * tiles, tile = q / nb, j = q - tile * nb;
   // blocks of nearly equal size
   const int r0 = static_cast<int>(static_cast<int64_t>(r.z) * j / nb), r1 = static_cast<int>(static_cast<int64_t>(r.z) * (j + 1) / nb);
@@ -118,9 +126,10 @@ template <bool UP, int STAGES, int ROWS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
     moe_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const MoeArgs A, int tiles) {
   using L = MLayout<STAGES, ROWS>;
-  constexpr bool ONCE = ROWS == MOE_BLOCK_ROWS_FEW;
+  constexpr bool ONCE = ROWS == MOE_BLOCK_ROWS_FEW, GATHER = UP && moe_gathers(ROWS);
   constexpr int BOX = 64;  // rows of a TMA box of B
-  auto box_count = [](int n) { return ((n + 15) / 16 * 8 + BOX - 1) / BOX; };
+  auto half_rows = [](int n) { return (n + 15) / 16 * 8; };  // a block's half of the MMA's N rows
+  auto box_count = [=](int n) { return (half_rows(n) + BOX - 1) / BOX; };
   extern __shared__ uint8_t dsmem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_addr(smem);
@@ -158,9 +167,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
   pair_sync();  // both blocks' barriers are set up and their TMEM is allocated
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // The plan is complete: the kernel before this one let it start only after its own wait for it. The weights' warp reads
-  // nothing else that a kernel wrote and starts at once.
+  // Behind another kernel than the plan itself, the plan is complete: that kernel let this one start only after its own wait
+  // for it. The weights' warp reads nothing else that a kernel wrote and starts at once.
+  if (GATHER) pdl_wait();
   const int nitems = __ldcg(&A.header->nblk) * tiles;
+  const int4 first = nitems > 0 ? moe_block(A, pair, tiles, nitems) : int4{};
   if (warp != 0) {
     pdl_wait();
     pdl_trigger();
@@ -171,10 +182,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
       const uint64_t policy = evict_first_policy();
       int kc = 0;
       bool ok = true;
+      int4 next = first;
       for (int it = pair; it < nitems && ok; it += npairs) {
-        const Item blk = moe_item(A, it, tiles);
+        const Item blk = moe_item(A, next, it, tiles);
+        next = moe_block(A, it + npairs, tiles, nitems);  // here long before it is used
         const int tile = blk.tile * 2 + static_cast<int>(rank);
-        const uint32_t bytes = 2 * (128 + box_count(blk.n) * BOX) * (SUB * MK * 2);
+        const uint32_t bytes = 2 * (128 + (GATHER ? half_rows(blk.n) : box_count(blk.n) * BOX)) * (SUB * MK * 2);
         for (int kt = 0; kt < k_tiles; ++kt, ++kc) {
           const int s = kc % STAGES;
           if (kc >= STAGES && !mbar_wait(empty_bar(s), ((kc / STAGES) - 1) & 1, abort_flag, A.err)) {
@@ -193,15 +206,59 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
       }
     }
     __syncwarp();
+  } else if (GATHER && warp >= 6) {
+    // Token rows by gathers of four; warp 6 takes the even ones, warp 7 the odd ones. Each has at least one in every stage: a
+    // warp with nothing to load would not be held by the ring and fall a turn behind.
+    static_assert(MTHREADS == 256, "two warps");
+    int s = 0;
+    uint32_t phase = 1;
+    bool ok = true;
+    static_assert(!GATHER || ROWS / 16 * 4 == 32, "a lane finds the token of one row");
+    auto place = [&](const Item& blk) {  // past the last: the first, whose column of the accumulator is not used
+      const int half = half_rows(blk.n), g = warp - 6 + lane / 4 * 2, r = static_cast<int>(rank) * half + g * 4 + lane % 4;
+      return __ldcg(A.rows + blk.row0 + (g < half / 4 && r < blk.n ? r : 0));
+    };
+    int4 next = first;
+    int mine = pair < nitems ? place(moe_item(A, next, pair, tiles)) : 0;
+    for (int it = pair; it < nitems && ok; it += npairs) {
+      const int gathers = half_rows(moe_item(A, next, it, tiles).n) / 4, token = mine / A.places;
+      next = moe_block(A, it + npairs, tiles, nitems);
+      int4 tok[ROWS / 16];
+#pragma unroll
+      for (int i = 0; i < ROWS / 16; ++i)
+        tok[i] = make_int4(__shfl_sync(0xffffffffu, token, 4 * i), __shfl_sync(0xffffffffu, token, 4 * i + 1),
+                           __shfl_sync(0xffffffffu, token, 4 * i + 2), __shfl_sync(0xffffffffu, token, 4 * i + 3));
+      for (int kt = 0; kt < k_tiles && ok; ++kt) {
+        ok = __all_sync(0xffffffffu, mbar_try(empty_bar(s), phase) || mbar_wait(empty_bar(s), phase, abort_flag, A.err));
+        if (!ok) break;
+        const uint32_t bar = mapa(full_bar(s), 0), b_s = sbase + s * L::STAGE_BYTES + L::A_BYTES;
+        if (elect_one()) {
+#pragma unroll
+          for (int i = 0; i < ROWS / 16; ++i)
+            if (warp - 6 + 2 * i < gathers)
+#pragma unroll
+              for (int j = 0; j < SUB; ++j)
+                pair_gather4(b_s + (j * ROWS / 2 + (warp - 6 + 2 * i) * 4) * MK * 2, &tmB, bar, (kt * SUB + j) * MK, tok[i]);
+        }
+        __syncwarp();
+        if (kt == 0 && it + npairs < nitems) mine = place(moe_item(A, next, it + npairs, tiles));
+        if (++s == STAGES) {
+          s = 0;
+          phase ^= 1;
+        }
+      }
+    }
   } else if (warp == 6) {
     if (lane == 0) {
       int kc = 0;
       bool ok = true;
+      int4 next = first;
       for (int it = pair; it < nitems && ok; it += npairs) {
-        const Item blk = moe_item(A, it, tiles);
+        const Item blk = moe_item(A, next, it, tiles);
+        next = moe_block(A, it + npairs, tiles, nitems);
         // this block's half of the MMA's N rows, in boxes of 64 (what lies past it is not read; boxes of 32 or 16
         // copy less and cost 6 and 20 % more where the MMAs bound the kernel: each box is an instruction)
-        const int nb = box_count(blk.n), row = blk.row0 + static_cast<int>(rank) * ((blk.n + 15) / 16 * 8);
+        const int nb = box_count(blk.n), row = blk.row0 + static_cast<int>(rank) * half_rows(blk.n);
         for (int kt = 0; kt < k_tiles; ++kt, ++kc) {
           const int s = kc % STAGES;
           if (kc >= STAGES && !mbar_wait(empty_bar(s), ((kc / STAGES) - 1) & 1, abort_flag, A.err)) {
@@ -226,8 +283,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
       const uint64_t desc = umma_desc(sbase);
       const uint32_t lo0 = static_cast<uint32_t>(desc), hi = static_cast<uint32_t>(desc >> 32);
       bool ok = true;
+      int4 next = first;
       for (int it = pair; it < nitems && ok; it += npairs, ++tc) {
-        const uint32_t idesc = umma_idesc_mn(256, (moe_item(A, it, tiles).n + 15) / 16 * 16);
+        const uint32_t idesc = umma_idesc_mn(256, half_rows(moe_item(A, next, it, tiles).n) * 2);
+        next = moe_block(A, it + npairs, tiles, nitems);
         const int buf = tc & 1;
         ok = __all_sync(0xffffffffu, tc < 2 || mbar_wait(acce_bar(buf), ((tc >> 1) - 1) & 1, abort_flag, A.err));
         tc_fence_after();
@@ -254,11 +313,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MTHREADS, 1)
       }
     }
     __syncwarp();
-  } else {
+  } else if (warp < 6) {
     const int q = warp & 3;  // TMEM lanes 32 q .. 32 q + 31
     int tc = 0;
     for (int it = pair; it < nitems; it += npairs, ++tc) {
-      const Item blk = moe_item(A, it, tiles);
+      const Item blk = moe_item(A, moe_block(A, it, tiles, nitems), it, tiles);
       const int tile = blk.tile * 2 + rank;
       const int buf = tc & 1;
       bool ok = mbar_wait(accf_bar(buf), (tc >> 1) & 1, abort_flag, A.err);
@@ -362,9 +421,10 @@ int moe_products_tc(const MoeArgs& A, int max_blocks, cudaStream_t s) {
     if ((rc = encode(&mgu, A.w_gu, 5, dims, strides, box)) != MMP_OK) return rc;
   }
   {
-    const u64 dims[2] = {H, R}, strides[1] = {H * 2};
-    const u32 box[2] = {MK, 64};
-    if ((rc = encode(&mx, A.xs, 2, dims, strides, box)) != MMP_OK) return rc;
+    const bool gather = moe_gathers(A.block_rows);
+    const u64 dims[2] = {H, gather ? static_cast<u64>(A.T) : R}, strides[1] = {(gather && A.T > 1 ? static_cast<u64>(A.x_t) : H) * 2};
+    const u32 box[2] = {MK, gather ? 1u : 64u};
+    if ((rc = encode(&mx, gather ? A.x : A.xs, 2, dims, strides, box)) != MMP_OK) return rc;
   }
   {
     const u64 dr = static_cast<u64>(A.d_r) * 2, de = A.E > 1 ? static_cast<u64>(A.d_e) * 2 : H * dr;
