@@ -13,7 +13,7 @@ namespace mmp {
 
 constexpr int MOE_MAX_EXPERTS = 1024;  // experts in the weight tensors (one thread each in the scan)
 constexpr int MOE_MAX_TOPK = 32;       // one lane each in the router
-constexpr int MOE_FEW_PLACES = 1536;   // the few-token kernels keep 16 fp32 a place in shared memory (96 KB)
+constexpr int MOE_FEW_PLACES = 1152;   // the few-token kernels keep 16 fp32 a place in shared memory (72 KB)
 constexpr int MOE_TINY_TOKENS = 8, MOE_TINY_PLACES = 64;  // up to which every block of the few-token kernels plans for itself
 // Sorted rows of one expert that the tensor-core kernels take at a time (MMA N): 256, or 128 with a deeper ring of weights
 // where experts have few rows.
@@ -47,10 +47,13 @@ struct MoeGroup {
 //   8 experts,   I 2048: 18 places 46 / 46, 64 52 / 46
 // The down product of the few-token kernels has a block for 16 columns of H, with few of them it does not fill the GPU:
 //   256 experts, H 1024, I 128: 128 places 27 / 35, 256 45 / 42;   I 512: 72 places 66 / 47
+// and with many it has two blocks an SM, beside which the results of more places do not fit:
+//   64 experts, H 7168, I 64: 512 places 65 / 89, 1024 145 / 96
+constexpr int MOE_WIDE = 16 * 148;
 inline bool moe_is_tiny(int64_t T, int places) { return T <= MOE_TINY_TOKENS && T * places <= MOE_TINY_PLACES; }
 inline bool moe_is_few(int64_t T, int places, int H, int I) {
   const int64_t R = T * places, w = std::min(H, 2048);
-  return moe_is_tiny(T, places) || (R <= MOE_FEW_PLACES && I <= 512 && R * I <= w * w / 64);
+  return moe_is_tiny(T, places) || (R <= (H <= MOE_WIDE ? MOE_FEW_PLACES : MOE_FEW_PLACES / 2) && I <= 512 && R * I <= w * w / 64);
 }
 
 // Workspace offsets in bytes, every part 256-byte aligned.
@@ -120,11 +123,12 @@ struct RouteParams {
 };
 
 // How the few-token kernels take a call: tiny (every block plans for itself, and routes where there are logits), rows of a
-// group.
+// group: 16 where few experts have many rows (us, 8 / 16: 16 experts, H 2048, I 128, 256 places 19.4 / 16.5; 8 experts, H 4096,
+// I 256, 64 places 24.6 / 17.2), 8 else (60 experts, H 2048, I 128, 512 places 32 / 39; 64, H 7168, I 128, 512 places 97 / 139).
 struct MoeFewPlan { bool tiny; int rows; };
 inline MoeFewPlan moe_few_plan(const MoeArgs& A) {
   const bool tiny = moe_is_tiny(A.T, A.places);
-  return {tiny, tiny || A.T * A.places <= 4 * A.E ? 8 : 16};
+  return {tiny, tiny || A.E > 32 || A.T * A.places <= 4 * A.E ? 8 : 16};
 }
 // The few-token products (moe_few.cu) and the sum into A.out.
 int moe_products_few(const MoeArgs& A, const RouteParams& P, bool f32, const MoeFewPlan& plan, cudaStream_t s);

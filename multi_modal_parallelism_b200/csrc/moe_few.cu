@@ -618,17 +618,15 @@ int launch_down(const MoeArgs& A, int limit, cudaStream_t s) {
   return MMP_OK;
 }
 
-// 16 warps while one block an SM covers the columns, else two blocks of 8; as long a queue as fits beside the results.
-static_assert(down_shared<8, 1, 2, 2>(MOE_FEW_PLACES, 1) <= SM_SHARED && down_shared<8, 1, 1, 2>(MOE_FEW_PLACES, 1) <= SM_SHARED,
-              "the last choices take any request");
+// 16 warps while one block an SM covers the columns, else two blocks of 8 while the results fit beside their queues.
+static_assert(down_shared<16, 1, 1, 3>(MOE_FEW_PLACES, 1) <= SM_SHARED && down_shared<8, 1, 2, 2>(MOE_FEW_PLACES, 1) <= SM_SHARED,
+              "there is a choice for any request");
 
 int products8(const MoeArgs& A, int max_groups, int sms, cudaStream_t s) {
   int rc = launch_up<1, 1>(A, max_groups, sms, s);
   if (rc != MMP_OK) return rc;
-  const int R = A.T * A.places, half = SM_SHARED / 2 - 1024;
-  if ((A.H + 15) / 16 <= sms && down_shared<16, 1, 1, 3>(R, 1) <= SM_SHARED) return launch_down<16, 1, 1, 3>(A, SM_SHARED, s);
-  if ((A.H + 15) / 16 > sms && down_shared<8, 1, 1, 3>(R, 1) <= half) return launch_down<8, 1, 1, 3>(A, half, s);
-  return launch_down<8, 1, 1, 2>(A, SM_SHARED, s);
+  if ((A.H + 15) / 16 <= sms) return launch_down<16, 1, 1, 3>(A, SM_SHARED, s);
+  return launch_down<8, 1, 1, 3>(A, std::max(SM_SHARED / 2 - 1024, down_shared<8, 1, 1, 3>(A.T * A.places, 1)), s);
 }
 
 int products16(const MoeArgs& A, int max_groups, int sms, cudaStream_t s) {
