@@ -162,3 +162,18 @@ def test_rope_axes():
             K.rope_axes(bad, False, dev)
     with pytest.raises(ValueError):
         K.rope_axes([1, 4, 4], True, dev)  # pairs of the other axes run out of places
+
+
+@pytest.mark.parametrize("T,places,H,I,E,launches", [
+    (1, 9, 2048, 512, 257, (1, 1)),         # one launch
+    (30, 4, 2048, 64, 16, (3, 3)),          # plan (with the routing of few tokens), up, down
+    (60, 4, 2048, 64, 16, (3, 4)),
+    (200, 4, 2048, 512, 16, (4, 5)),        # plan, up, down, sum
+    (2000, 4, 2048, 512, 16, (5, 6)),       # plan, sorted rows, up, down, sum
+])
+def test_launches_and_scratch(T, places, H, I, E, launches):
+    lib = _lib.lib()
+    assert tuple(lib.mmp_moe_launches(T, places, H, I, E, r) for r in (0, 1)) == launches
+    # the scratch of a request serves every smaller one
+    sizes = [lib.mmp_moe_workspace_size(t, places, H, I, E) for t in range(1, T + 1)]
+    assert sizes == sorted(sizes)
