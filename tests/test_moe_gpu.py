@@ -174,15 +174,15 @@ def test_experts_many_tokens(T, E, k, H, I):
     check_experts(K.moe_experts(*a[:5], addend=a[5]), *a)
 
 
-@pytest.mark.parametrize("T,E,k,H,I", [(100, 16, 2, 512, 96), (1000, 16, 2, 512, 96)])
+@pytest.mark.parametrize("T,E,k,H,I", [(20, 16, 2, 512, 96), (100, 16, 2, 512, 96), (1000, 16, 2, 512, 96)])
 def test_experts_all_tokens_on_the_same_experts(T, E, k, H, I):
     a = make(T, E, k, H, I, skew=True)
     check_experts(K.moe_experts(*a[:5], addend=a[5]), *a)
 
 
-@pytest.mark.parametrize("T", [40, 1100])
+@pytest.mark.parametrize("T", [40, 200, 1100])
 def test_experts_without_addend_and_rows_without_experts(T):
-    a = make(T, 16, 4, 256, 64, pad=7)
+    a = make(T, 16, 4, 1024, 64, pad=7)
     a[4][3] = -1           # a whole row
     a[4][5, 1:] = -1       # some of its places
     a[4][6, 1] = a[4][6, 0]  # the same expert twice
@@ -194,16 +194,16 @@ def test_experts_without_addend_and_rows_without_experts(T):
     assert torch.equal(out[3], a[5][3]) and torch.equal(out[-7:], a[5][-7:])
 
 
-@pytest.mark.parametrize("T", [3, 1000])
+@pytest.mark.parametrize("T", [3, 20, 100, 1000])
 def test_experts_no_places_at_all(T):
-    a = make(T, 8, 2, 128, 64)
+    a = make(T, 8, 2, 512, 64)
     a[4].fill_(-1)
     assert torch.equal(K.moe_experts(*a[:5], addend=a[5]), a[5])
 
 
-@pytest.mark.parametrize("T", [10, 1000])
+@pytest.mark.parametrize("T", [4, 10, 100, 1000])
 def test_experts_index_out_of_range_is_reported_and_adds_nothing(T):
-    a = make(T, 8, 2, 128, 64)
+    a = make(T, 8, 2, 512, 64)
     ids = a[4].clone()
     a[4][1, 0] = 8
     ids[1, 0] = -1
@@ -213,9 +213,9 @@ def test_experts_index_out_of_range_is_reported_and_adds_nothing(T):
     check_experts(out, a[0], a[1], a[2], a[3], ids, a[5])
 
 
-@pytest.mark.parametrize("T", [10, 1000])
+@pytest.mark.parametrize("T", [10, 100, 1000])
 def test_experts_strided_rows_and_out_over_the_addend(T):
-    E, k, H, I = 8, 2, 136, 72
+    E, k, H, I = 8, 2, 520, 72
     a = make(T, E, k, H, I)
     x = torch.zeros(T, H + 24, dtype=BF, device=DEV)[:, 8:8 + H].copy_(a[0])
     wgu = torch.zeros(E, 2 * I + 3, H + 8, dtype=BF, device=DEV)[:, :2 * I, :H].copy_(a[1])
@@ -229,9 +229,9 @@ def test_experts_strided_rows_and_out_over_the_addend(T):
     assert bool((guard[:, :8] == 7).all()) and bool((guard[:, 8 + H:] == 7).all())
 
 
-@pytest.mark.parametrize("T", [24, 1000])
+@pytest.mark.parametrize("T", [24, 60, 1000])
 def test_experts_non_finite_token_stays_in_its_row(T):
-    a = make(T, 4, 2, 128, 64)
+    a = make(T, 4, 2, 512, 64)
     clean = K.moe_experts(*a[:5], addend=a[5])
     a[0][5, 3] = math.nan
     a[0][7, 3] = INF
@@ -241,9 +241,9 @@ def test_experts_non_finite_token_stays_in_its_row(T):
     assert torch.equal(out[keep], clean[keep]) and bool(torch.isnan(out[5]).all())
 
 
-@pytest.mark.parametrize("T", [16, 1000])
+@pytest.mark.parametrize("T", [16, 100, 1000])
 def test_experts_same_bits_every_time(T):
-    a = make(T, 16, 4, 512, 128)
+    a = make(T, 16, 4, 1024, 128)
     first = K.moe_experts(*a[:5], addend=a[5])
     for _ in range(5):
         assert torch.equal(K.moe_experts(*a[:5], addend=a[5]), first)
@@ -261,7 +261,8 @@ def test_empty_batch():
 # ------------------------------------------------------------------------------------------------ layer
 @pytest.mark.parametrize("dtype", [torch.float32, BF])
 @pytest.mark.parametrize("T,E,k,H,I,shared", [(1, 16, 4, 256, 64, True), (7, 256, 8, 512, 128, True), (64, 40, 6, 264, 72, False),
-                                              (200, 8, 2, 128, 64, True), (700, 16, 4, 256, 128, True), (1700, 30, 1, 64, 32, False)])
+                                              (200, 8, 2, 128, 64, True), (700, 16, 4, 256, 128, True), (1700, 30, 1, 64, 32, False),
+                                              (20, 16, 4, 1024, 64, True), (60, 16, 4, 2048, 64, True)])
 def test_layer_is_route_and_experts(dtype, T, E, k, H, I, shared):
     n = E + shared
     x, wgu, wd, _, _, add = make(T, n, 1, H, I, seed=E)
@@ -277,9 +278,9 @@ def test_layer_is_route_and_experts(dtype, T, E, k, H, I, shared):
     assert torch.equal(K.moe_experts(x, wgu, wd, w2, ids2, addend=add), out)
 
 
-@pytest.mark.parametrize("T", [8, 600])
+@pytest.mark.parametrize("T", [8, 40, 200, 600])
 def test_layer_captured_and_replayed_on_new_inputs(T):
-    E, k, H, I = 16, 4, 256, 64
+    E, k, H, I = 16, 4, 1024, 64
     x, wgu, wd, _, _, add = make(T, E + 1, 1, H, I)
     l = torch.randn(T, E + 1, device=DEV, generator=gen(2)).to(BF)
     out = torch.empty(T, H, dtype=BF, device=DEV)
@@ -298,10 +299,10 @@ def test_layer_captured_and_replayed_on_new_inputs(T):
         assert torch.equal(replayed, K.moe_layer(x, l, wgu, wd, k, shared=True, addend=add))
 
 
-@pytest.mark.parametrize("T", [8, 600])
+@pytest.mark.parametrize("T", [8, 20, 100, 600])
 def test_two_streams_at_once(T):
     """Calls on two streams overlap; each has scratch of its own when none is given."""
-    a, b = make(T, 16, 4, 512, 128, seed=1), make(T, 16, 4, 512, 128, seed=2)
+    a, b = make(T, 16, 4, 1024, 128, seed=1), make(T, 16, 4, 1024, 128, seed=2)
     want = [K.moe_experts(*q[:5], addend=q[5]) for q in (a, b)]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream(DEV) for _ in range(2)]
@@ -316,10 +317,10 @@ def test_two_streams_at_once(T):
 
 
 @pytest.mark.parametrize("renorm", [True, False])
-@pytest.mark.parametrize("T", [5, 40, 700])
+@pytest.mark.parametrize("T", [5, 40, 200, 700])
 def test_layer_rows_whose_mask_leaves_nothing(T, renorm):
     """A token with every expert masked gets the addend alone, with the shared expert that one's share."""
-    E, k, H, I = 16, 4, 256, 64
+    E, k, H, I = 16, 4, 1024, 64
     x, wgu, wd, _, _, add = make(T, E + 1, 1, H, I)
     l = torch.randn(T, E + 1, device=DEV, generator=gen(4)).to(BF)
     l[[1, T - 1], :E] = -INF
@@ -337,7 +338,7 @@ def test_layer_rows_whose_mask_leaves_nothing(T, renorm):
 
 def test_one_scratch_for_calls_of_every_path_in_a_row():
     """Calls that follow one another on a stream share one scratch, sized for the largest; none is waited for."""
-    E, k, H, I = 16, 4, 512, 128
+    E, k, H, I = 16, 4, 2048, 128
     batches = [3, 900, 40, 8, 1500, 200, 1, 64]
     data = [make(T, E, k, H, I, seed=T) for T in batches]
     want = [K.moe_experts(*a[:5], addend=a[5]) for a in data]
@@ -349,9 +350,9 @@ def test_one_scratch_for_calls_of_every_path_in_a_row():
         assert torch.equal(g, w)
 
 
-@pytest.mark.parametrize("T", [8, 40, 600])
+@pytest.mark.parametrize("T", [8, 40, 200, 600])
 def test_two_captured_graphs_with_a_scratch_each(T):
-    E, k, H, I = 16, 4, 256, 64
+    E, k, H, I = 16, 4, 1024, 64
     data = [make(T, E, k, H, I, seed=s) for s in (1, 2)]
     want = [K.moe_experts(*a[:5], addend=a[5]) for a in data]
     graphs, outs, streams = [], [], [torch.cuda.Stream(DEV) for _ in data]
@@ -375,8 +376,8 @@ def test_two_captured_graphs_with_a_scratch_each(T):
 
 def test_chained_layers_read_what_the_one_before_wrote():
     """Each call's output is the next one's input, on every path, without a wait: the same bits as with one."""
-    E, k, H, I = 16, 4, 256, 64
-    for T in (8, 40, 600):
+    E, k, H, I = 16, 4, 1024, 64
+    for T in (8, 40, 200, 600):
         x, wgu, wd, w, ids, _ = make(T, E, k, H, I, seed=T)
         y = x
         for _ in range(6):
