@@ -56,7 +56,7 @@ __device__ __forceinline__ void pair_gather4(uint32_t dst, const CUtensorMap* ma
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w) : "memory");
 }
 // Weights: ONCE where most experts have one row block, so that they are the first to leave L2 (777 tokens x 4 of 60 experts
-// 199 -> 193 us; with several blocks an expert they are read again: 2 of 8 large experts 1164 -> 1227 us).
+// 199 -> 193 us; with several blocks an expert they are read again: 4096 tokens x 2 of 8 large experts 1078 -> 1106 us).
 template <bool ONCE>
 __device__ __forceinline__ void pair_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, uint64_t policy) {
   if constexpr (!ONCE) {
