@@ -126,17 +126,30 @@ def advance_decode_ctx(ctx: DecodeCtx, n: int = 1) -> None:
     ctx.max_k += n
 
 
+def _rotary_after(pc: PrefillCtx) -> torch.Tensor:
+    """[axes, nseq]: the rotary positions of the token after each sequence's rows of a prefill with several axes."""
+    if tuple(pc.positions.shape[1:]) != (pc.T,):
+        raise ValueError(f"decode_ctx_after: positions {tuple(pc.positions.shape)} are not [axes, {pc.T}]")
+    if any(s > 0 and L == 0 for s, L in zip(pc.starts, pc.lens)):
+        raise ValueError("decode_ctx_after: a sequence with cached and without new tokens has no rotary position to go on from")
+    per = pc.positions.cpu().split(list(pc.lens), dim=1)
+    nxt = torch.tensor([int(p.max()) + 1 if p.shape[1] else 0 for p in per], dtype=torch.int64)
+    return nxt.repeat(pc.positions.shape[0], 1)
+
+
 def decode_ctx_after(pc: PrefillCtx) -> DecodeCtx:
     """The decode step that follows a prefill: one new token per sequence at position starts[i] + lens[i],
-    same block table and state lines."""
+    same block table and state lines. After rotary positions with several axes the new token's are, on every axis,
+    one past the largest of its sequence's rows in `pc`; where it is cached still follows its index."""
     tot = torch.tensor([s + L for s, L in zip(pc.starts, pc.lens)], dtype=torch.int64)
     table = pc.block_table.cpu()
     if int(tot.max()) // pc.kv_block >= table.shape[1]:
         raise ValueError("decode_ctx_after: no cache block reserved for the next token")
     slot = table[torch.arange(pc.nseq), tot // pc.kv_block].to(torch.int64) * pc.kv_block + tot % pc.kv_block
     dev = pc.block_table.device
+    pos = tot if pc.positions.dim() == 1 else _rotary_after(pc)
     return DecodeCtx(
-        B=pc.nseq, c=int(tot.max()), kv_block=pc.kv_block, nblk=table.shape[1], positions=tot.to(dev),
+        B=pc.nseq, c=int(tot.max()), kv_block=pc.kv_block, nblk=table.shape[1], positions=pos.to(dev),
         cu_q=torch.arange(pc.nseq + 1, dtype=torch.int32).to(dev), seqused_k=(tot + 1).to(torch.int32).to(dev),
         block_table=pc.block_table, slot_mapping=slot.to(dev), state_idx=pc.state_idx, max_k=int(tot.max()) + 1,
     )

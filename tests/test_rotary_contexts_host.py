@@ -1,0 +1,61 @@
+"""Contexts whose rotary positions have several axes ([axes, rows]): a decode context that follows such a prefill goes on from
+its rotary positions, not from the tokens' places in the cache (state.decode_ctx_after, advance_decode_ctx)."""
+import dataclasses
+
+import pytest
+import torch
+
+from multi_modal_parallelism_b200.state import advance_decode_ctx, decode_ctx_after, make_prefill_ctx
+
+CPU = torch.device("cpu")
+
+
+def image_prefill(lens, starts=None, base=0):
+    """Per sequence three text tokens, then rows of a grid four wide whose time stands still, all from `base` on."""
+    pc = make_prefill_ctx(list(lens), 16, CPU, starts=starts, reserve=8)
+    per = []
+    for n in lens:
+        t = torch.arange(n)
+        grid = torch.stack([torch.full((n,), 3), 3 + (t - 3) // 4, 3 + (t - 3) % 4])
+        per.append(torch.where(t < 3, t, grid) + base)
+    return dataclasses.replace(pc, positions=torch.cat(per, 1)), per
+
+
+@pytest.mark.parametrize("lens", [(12,), (5, 30, 3, 1)])
+def test_decode_after_several_axes_goes_on_from_the_largest_position(lens):
+    pc, per = image_prefill(lens)
+    dc = decode_ctx_after(pc)
+    want = torch.stack([p.max() + 1 for p in per]).expand(3, -1)
+    assert dc.positions.dtype == torch.int64 and torch.equal(dc.positions, want)
+    # where the token is cached and how many keys it sees follow its index, not its rotary position
+    flat = decode_ctx_after(dataclasses.replace(pc, positions=make_prefill_ctx(list(lens), 16, CPU, reserve=8).positions))
+    assert flat.positions.tolist() == list(lens)
+    for name in ("slot_mapping", "seqused_k", "block_table", "state_idx", "cu_q"):
+        assert torch.equal(getattr(dc, name), getattr(flat, name)), name
+    assert (dc.c, dc.max_k, dc.B) == (flat.c, flat.max_k, flat.B)
+    advance_decode_ctx(dc)
+    advance_decode_ctx(flat)
+    assert torch.equal(dc.positions, want + 1) and torch.equal(dc.slot_mapping, flat.slot_mapping)
+
+
+def test_decode_after_a_continued_prefill_with_several_axes():
+    pc, per = image_prefill((7, 12), starts=[20, 4], base=50)
+    dc = decode_ctx_after(pc)
+    assert torch.equal(dc.positions, torch.stack([p.max() + 1 for p in per]).expand(3, -1))
+    assert dc.seqused_k.tolist() == [28, 17]
+
+
+def test_sequences_without_new_tokens():
+    """A fresh sequence without tokens starts at position 0; one that has cached tokens and no new ones gives no rotary
+    position to go on from."""
+    pc, per = image_prefill((7, 0))
+    assert decode_ctx_after(pc).positions.tolist() == [[int(per[0].max()) + 1, 0]] * 3
+    pc, _ = image_prefill((7, 0), starts=[0, 5])
+    with pytest.raises(ValueError, match="rotary position"):
+        decode_ctx_after(pc)
+
+
+def test_positions_that_do_not_cover_the_rows_are_refused():
+    pc, _ = image_prefill((7, 5))
+    with pytest.raises(ValueError, match="positions"):
+        decode_ctx_after(dataclasses.replace(pc, positions=pc.positions[:, :-1]))
