@@ -213,10 +213,16 @@ class _Mlp:
 class _Moe:
     """Mixture of experts over this rank's columns of every expert: the router's product, then routing, the experts'
     products and their weighted sum (a partial sum when the columns are split; every rank routes alike). The shared
-    expert is the last of the experts, its gate the last of the router's rows."""
+    expert is the last of the experts, its gate the last of the router's rows. ws: scratch of up to `rows` tokens, which
+    layers that run one after another share."""
 
-    def __init__(self, d: Qwen35Dims, w: dict, cols: range, device: torch.device, rows: int):
-        self.d, n, I = d, cols.stop - cols.start, d.moe_intermediate
+    @staticmethod
+    def scratch(d: Qwen35Dims, cols: range, device: torch.device, rows: int) -> torch.Tensor:
+        shared = int(d.shared_expert)
+        return K.moe_workspace(rows, d.top_k + shared, d.hidden, cols.stop - cols.start, d.n_experts + shared, device)
+
+    def __init__(self, d: Qwen35Dims, w: dict, cols: range, device: torch.device, rows: int, ws: torch.Tensor):
+        self.d, self.ws, I = d, ws, d.moe_intermediate
         sl, su = slice(cols.start, cols.stop), slice(I + cols.start, I + cols.stop)
         router, gu, down = w["mlp.gate.weight"], w["mlp.experts.gate_up_proj"], w["mlp.experts.down_proj"]
         gu, down = torch.cat([gu[:, sl], gu[:, su]], 1), down[:, :, sl]
@@ -228,7 +234,6 @@ class _Moe:
         self.w_router, self.w_gu, self.w_down = _put(router, device), _put(gu, device), _put(down, device)
         E = self.w_down.shape[0]
         self.logits = torch.empty(rows, _pad8(E), device=device, dtype=BF16)
-        self.ws = K.moe_workspace(rows, d.top_k + d.shared_expert, d.hidden, n, E, device)
 
     def forward(self, y: torch.Tensor, out: torch.Tensor, addend: torch.Tensor | None = None) -> torch.Tensor:
         logits = K.gemm(y, self.w_router, out=self.logits[:y.shape[0], :self.w_router.shape[0]])
@@ -239,13 +244,13 @@ class _Moe:
 class _Layer:
     """Norm, mixer, collective, residual + norm, MLP, collective, residual."""
 
-    def __init__(self, d: Qwen35Dims, w: dict, groups: Groups, device: torch.device, rows: int):
+    def __init__(self, d: Qwen35Dims, w: dict, groups: Groups, device: torch.device, rows: int, moe_ws: torch.Tensor | None):
         self.d, self.groups, self.device = d, groups, device
         self.world = groups.world_size
         self.in_norm = _put(w["input_layernorm.weight"], device)
         self.post_norm = _put(w["post_attention_layernorm.weight"], device)
         cols = mlp_cols(d, groups.rank, self.world)
-        self.mlp = _Moe(d, w, cols, device, rows) if d.n_experts else _Mlp(w, cols, device, rows)
+        self.mlp = _Moe(d, w, cols, device, rows, moe_ws) if d.n_experts else _Mlp(w, cols, device, rows)
         mk = lambda: torch.empty(rows, d.hidden, device=device, dtype=BF16)  # noqa: E731
         self.xn, self.mix, self.h1, self.y, self.part, self.out = mk(), mk(), mk(), mk(), mk(), mk()
 
@@ -270,8 +275,9 @@ class _Layer:
 class GdnLayer(_Layer):
     """Gated delta-rule layer on this rank's key/value heads (tp over all ranks in every layout)."""
 
-    def __init__(self, d: Qwen35Dims, w: dict, groups: Groups, device: torch.device, rows: int, lines: int):
-        super().__init__(d, w, groups, device, rows)
+    def __init__(self, d: Qwen35Dims, w: dict, groups: Groups, device: torch.device, rows: int, lines: int,
+                 moe_ws: torch.Tensor | None = None):
+        super().__init__(d, w, groups, device, rows, moe_ws)
         sh = gdn_shard(d, groups.rank, self.world)
         self.shard = sh
         self.nk, self.nv = len(sh.k_heads), len(sh.v_heads)
@@ -353,8 +359,8 @@ class AttnLayer(_Layer):
     (all heads; this rank's block of sequences; outputs all-gathered)."""
 
     def __init__(self, d: Qwen35Dims, w: dict, groups: Groups, device: torch.device, rows: int, num_blocks: int,
-                 kv_block: int, dp: bool):
-        super().__init__(d, w, groups, device, rows)
+                 kv_block: int, dp: bool, moe_ws: torch.Tensor | None = None):
+        super().__init__(d, w, groups, device, rows, moe_ws)
         self.dp = dp and self.world > 1
         sh = AttnShard(range(d.n_q), range(d.n_kv)) if self.dp else attn_shard(d, groups.rank, self.world)
         self.shard = sh
@@ -437,7 +443,8 @@ class AttnLayer(_Layer):
 
 class Qwen35Stack:
     """The layer stack on this rank. `lines` state lines per delta-rule layer (line 0 the null line),
-    `num_blocks` KV blocks of `kv_block` tokens per attention layer, `max_tokens` rows per call."""
+    `num_blocks` KV blocks of `kv_block` tokens per attention layer, `max_tokens` rows per call. Steps of one stack
+    must not overlap on the GPU: they share its buffers, and the layers one scratch for their experts."""
 
     def __init__(self, d: Qwen35Dims, weights: list[dict], mode: str, groups: Groups, device: torch.device,
                  lines: int, num_blocks: int, kv_block: int, max_tokens: int):
@@ -447,11 +454,12 @@ class Qwen35Stack:
             raise ValueError(f"Qwen35Stack: {len(weights)} weight sets for layout {d.layout!r}")
         self.d, self.mode, self.groups = d, mode, groups
         self.layers: list[_Layer] = []
+        ws = _Moe.scratch(d, mlp_cols(d, groups.rank, groups.world_size), device, max_tokens) if d.n_experts else None
         for kind, w in zip(d.layout, weights):
             if kind == "G":
-                self.layers.append(GdnLayer(d, w, groups, device, max_tokens, lines))
+                self.layers.append(GdnLayer(d, w, groups, device, max_tokens, lines, ws))
             else:
-                self.layers.append(AttnLayer(d, w, groups, device, max_tokens, num_blocks, kv_block, mode == "attn_dp"))
+                self.layers.append(AttnLayer(d, w, groups, device, max_tokens, num_blocks, kv_block, mode == "attn_dp", ws))
 
     def step(self, h: torch.Tensor, ctx) -> torch.Tensor:
         """One prefill (ctx a PrefillCtx: h [T, H] packed sequences) or decode step (ctx a DecodeCtx: h [B, H])
