@@ -47,9 +47,8 @@ class AttentionBranch:
         (the fused projections of a rank that holds both)."""
         a = plan.attn
         assert a is not None
-        if ctx.positions.dim() != 1:
-            raise ValueError(f"AttentionBranch: positions {tuple(ctx.positions.shape)} for a rotation with one axis")
-        self.plan, self.w, self.dims, self.st, self.ctx = plan, w, dims, st, ctx
+        self.bind(ctx)
+        self.plan, self.w, self.dims, self.st = plan, w, dims, st
         self.nq, self.nkv, self.hd = len(a.q_heads), len(a.kv_heads), dims.head_dim
         self.inv_freq = K.rope_inv_freq(self.hd, dims.rope_theta, device)
         self.prefill = isinstance(ctx, PrefillCtx)
@@ -62,6 +61,11 @@ class AttentionBranch:
         if not self.prefill:
             self.splits = K.attn_default_splits(B, self.nkv, ctx.max_k)
             self.ws = K.attn_workspace(B, self.nq, self.hd, self.splits, device)
+
+    def bind(self, ctx) -> None:
+        if ctx.positions.dim() != 1:
+            raise ValueError(f"AttentionBranch: positions {tuple(ctx.positions.shape)} for a rotation with one axis")
+        self.ctx = ctx
 
     @property
     def rope_cache(self) -> torch.Tensor:
@@ -406,10 +410,11 @@ class ParallelHybridLayer:
             self.s_ssm = torch.cuda.Stream(device=device)
 
     def _bind(self, ctx) -> None:
+        if self.attn is not None:
+            self.attn.bind(ctx)
+        if self.ssm is not None:
+            self.ssm.ctx = ctx
         self.ctx = ctx
-        for br in (self.attn, self.ssm):
-            if br is not None:
-                br.ctx = ctx
 
     def set_prefill_options(self, ssd_segments: bool) -> None:
         """Change how later prefills run (the balanced-walk SSD scan on or off); drops the per-shape prefill

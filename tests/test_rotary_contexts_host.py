@@ -59,3 +59,31 @@ def test_positions_that_do_not_cover_the_rows_are_refused():
     pc, _ = image_prefill((7, 5))
     with pytest.raises(ValueError, match="positions"):
         decode_ctx_after(dataclasses.replace(pc, positions=pc.positions[:, :-1]))
+
+
+def test_one_axis_layer_refuses_several_axes_on_every_prefill(monkeypatch):
+    """Also where the buffers for that many rows are there already from a prefill with one axis."""
+    from multi_modal_parallelism_b200 import layer as L
+    from multi_modal_parallelism_b200.config import preset
+    from multi_modal_parallelism_b200.dist import Coordinator, Groups
+    from multi_modal_parallelism_b200.sharding import plan_for
+    from multi_modal_parallelism_b200.state import alloc_states
+    from multi_modal_parallelism_b200.weights import random_layer, shard_to_device
+    from tests import _kernel_stand_ins as S
+
+    monkeypatch.setattr(L, "K", S)
+    dims = preset("hybrid_small")
+    plan = plan_for("tp1", 0, 1, dims)
+    pc = make_prefill_ctx([6, 3], 16, CPU)
+    st = alloc_states(plan, dims, 3, pc.block_table.numel(), 16, CPU, torch.float32)
+    groups = Groups(rank=0, local_rank=0, world_size=1, tp=Coordinator((0,), None), pair=None, device=CPU)
+    layer = L.ParallelHybridLayer(plan, shard_to_device(random_layer(dims, 0), plan, dims, CPU), dims, groups, st,
+                                  decode_ctx_after(pc), CPU, overlap_branches=False)
+    h = torch.randn(9, dims.hidden, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16)
+    several = dataclasses.replace(pc, positions=pc.positions.expand(3, -1))
+    with pytest.raises(ValueError, match="one axis"):
+        layer.prefill(h, several)
+    first = layer.prefill(h, pc).clone()
+    with pytest.raises(ValueError, match="one axis"):
+        layer.prefill(h, several)
+    assert torch.equal(layer.prefill(h, pc), first)
