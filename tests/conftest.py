@@ -37,3 +37,21 @@ def pytest_collection_modifyitems(config, items):
     for it in items:
         if "gpu" in it.keywords:
             it.add_marker(skip)
+
+
+def _stood_in():
+    """The package's modules whose `K` is not the kernels module."""
+    K = sys.modules.get("multi_modal_parallelism_b200.kernels")
+    return [m for n, m in list(sys.modules.items()) if n.startswith("multi_modal_parallelism_b200.") and K is not None
+            and getattr(m, "K", K) is not K]
+
+
+@pytest.fixture(autouse=True)
+def _kernels_module(request):
+    """Host tests may assign stand-ins for the kernels module (`qwen35.K = ...`): they end with the test, and no GPU test starts
+    with one."""
+    if request.node.get_closest_marker("gpu"):
+        assert not _stood_in(), [m.__name__ for m in _stood_in()]
+    yield
+    for m in _stood_in():
+        m.K = sys.modules["multi_modal_parallelism_b200.kernels"]
