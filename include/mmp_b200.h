@@ -139,7 +139,8 @@ int mmp_rope_kv_write(const void* q, int64_t q_b, const void* k, int64_t k_b, co
  * The several-axis form of mmp_rope_kv_write (no counterpart in the reference, whose positions have one axis): tokens of
  * images and video carry a position for each axis (time, height, width). qkv: [T, (nq + 2 nkv) hd] bf16 rows [q | k | v]
  * with row stride `row`. Pair i < rd / 2 of a head (dims i and i + rd / 2; dims >= rd are not rotated) of q and of
- * key_mult * k turns by positions[axes[i], t] * inv_freq[i], the product taken exactly (far positions keep their angle).
+ * key_mult * k turns by positions[axes[i], t] * inv_freq[i], right to fp32's rounding of the angle within one turn while
+ * |position| < 2^53 (far positions keep their angle).
  * positions: [naxes, T] int64, rows of stride p_a (0: one row for all axes); inv_freq, axes: [rd / 2] fp32 / int32 (an axis
  * outside [0, naxes) sets MMP_DEVERR_INDEX and counts as axis 0). q goes to q_out [T, nq hd] (row stride qo_b; may be the q part of qkv itself);
  * key_mult * k, rotated, and v go to the caches at slot_mapping[t] (neither where it is < 0; a slot past the cache sets

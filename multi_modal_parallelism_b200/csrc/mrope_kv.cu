@@ -2,8 +2,9 @@
 // one pass over the QKV projection. Pair i of the rd / 2 rotated pairs (dims i and i + rd / 2; dims from rd on pass) turns by
 //   angle = positions[axes[i], t] * inv_freq[i].
 //
-// The product is taken in fp64 and reduced by whole turns before sincosf: in fp32 the angle of position 10^6 would be off by
-// up to 0.03. One block a token: rd / 2 threads fill the token's cos/sin table once for all its heads (the single-axis kernel
+// The product is taken as a sum of two doubles and reduced by whole turns (2 pi in two parts, after Cody and Waite) before
+// sincosf: in fp32 the angle of position 10^6 would be off by up to 0.03, in fp64 alone that of 10^10 by 1.3e-6, of 10^12 by
+// 1.3e-4. One block a token: rd / 2 threads fill the token's cos/sin table once for all its heads (the single-axis kernel
 // computes them for every head), then every thread moves 16 + 16 bytes of a rotated head, or 16 of a passing or value part, at
 // a time. Bound by HBM (each value is read once and written once): 403 MB for 16384 tokens of 48 heads x 128 in 69 us, 5.8 TB/s.
 #include "mmp_common.cuh"
@@ -27,10 +28,12 @@ struct MropeParams {
 };
 
 __device__ __forceinline__ float2 turn(int64_t pos, float freq) {
-  constexpr double TAU = 6.283185307179586476925;
-  const double a = static_cast<double>(pos) * static_cast<double>(freq);
+  // 2 pi rounded to fp64 and what that leaves of it, 1 / (2 pi)
+  constexpr double TAU = 6.283185307179586476925, TAU_REST = 2.4492935982947064e-16, TURNS = 0.15915494309189533577;
+  const double p = static_cast<double>(pos), f = static_cast<double>(freq);  // exact below 2^53
+  const double a = p * f, rest = fma(p, f, -a), k = rint(a * TURNS);
   float s, c;
-  sincosf(static_cast<float>(a - rint(a / TAU) * TAU), &s, &c);
+  sincosf(static_cast<float>(fma(-k, TAU_REST, fma(-k, TAU, a) + rest)), &s, &c);
   return make_float2(c, s);
 }
 

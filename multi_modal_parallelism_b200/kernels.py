@@ -295,7 +295,7 @@ def qkv_mrope_kv_write(qkv: torch.Tensor, nq: int, nkv: int, head_dim: int, posi
     """qkv_rope_kv_write for positions with several axes (time, height, width): positions [naxes, T] int64; pair i of a head
     (dims i and i + rd/2, rd = 2 * inv_freq.numel() <= head_dim; the dims from rd on pass unrotated) turns by
     positions[axes[i], t] * inv_freq[i] (axes from rope_axes). Rows with slot_mapping < 0 are rotated into q_out and not
-    cached. Angles are exact at any position."""
+    cached. Angles are right to fp32's rounding (of the angle within one turn) while |position| < 2^53."""
     name = "qkv_mrope_kv_write"
     d = _device(name, qkv, positions, inv_freq, axes, q_out, key_cache, value_cache, slot_mapping)
     if not qkv.dtype == q_out.dtype == key_cache.dtype == value_cache.dtype == BF16:
