@@ -813,6 +813,8 @@ def _moe_args(name: str, x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch
         add = addend.data_ptr()
     if workspace is None:
         workspace = torch.empty(_moe_workspace_bytes(T, places, H, I, E), dtype=torch.uint8, device=x.device)
+    elif not workspace.is_contiguous():  # its size below is that of the memory behind it
+        raise ValueError(f"{name}: workspace must be contiguous, got {tuple(workspace.shape)} strides {workspace.stride()}")
     return (T, H, I, E, x_t, (w_gate_up.data_ptr(), gu[0], gu[1], w_down.data_ptr(), dn[0], dn[1]),
             (add, a_t, out.data_ptr(), o_t), out, workspace, workspace.numel() * workspace.element_size())
 
