@@ -372,6 +372,8 @@ class AttnLayer(_Layer):
                                     w["self_attn.v_proj.weight"][ks]]), device)
         self.wo = _put(w["self_attn.o_proj.weight"][:, qs], device)
         rd = d.rotary_dim or hd
+        if not 0 < rd <= hd or rd % 2:
+            raise ValueError(f"AttnLayer: rotary_dim {d.rotary_dim} must be even and at most head_dim {hd}")
         self.inv_freq = K.rope_inv_freq(rd, d.rope_theta, device)
         sections = tuple(d.rope_sections) or ((rd // 2,) if rd < hd else ())
         if sections and sum(sections) != rd // 2:

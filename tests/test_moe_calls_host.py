@@ -26,3 +26,19 @@ def test_scratch_with_gaps_or_repeats_is_refused(cpu, scratch):  # noqa: F811
         K.moe_experts(**experts(workspace=scratch))
     with pytest.raises(ValueError, match="workspace"):
         K.moe_layer(a["x"], torch.zeros(T, E), a["w_gate_up"], a["w_down"], k, workspace=scratch)
+
+
+@pytest.mark.parametrize("rotary", [-2, 1, 63, 65, 130, 128])
+def test_rotation_of_more_dims_than_a_head_or_of_an_odd_number_is_refused(monkeypatch, rotary):
+    from multi_modal_parallelism_b200 import qwen35 as Q
+    from multi_modal_parallelism_b200.dist import Coordinator, Groups
+    from tests import _kernel_stand_ins as S
+
+    monkeypatch.setattr(Q, "K", S)
+    dev = torch.device("cpu")
+    g = Groups(rank=0, local_rank=0, world_size=1, tp=Coordinator((0,), None), pair=None, device=dev)
+    d = Q.Qwen35Dims(hidden=256, n_q=4, n_kv=2, head_dim=64, intermediate=64, layout="A")
+    for ok in (0, 2, 32, 64):
+        Q.Qwen35Stack(d.replace(rotary_dim=ok), Q.random_stack(d, 0), "tp", g, dev, 2, 4, 16, 8)
+    with pytest.raises(ValueError, match="rotary_dim"):
+        Q.Qwen35Stack(d.replace(rotary_dim=rotary), Q.random_stack(d, 0), "tp", g, dev, 2, 4, 16, 8)
