@@ -63,8 +63,8 @@ class AttentionBranch:
             self.ws = K.attn_workspace(B, self.nq, self.hd, self.splits, device)
 
     def bind(self, ctx) -> None:
-        if ctx.positions.dim() != 1:
-            raise ValueError(f"AttentionBranch: positions {tuple(ctx.positions.shape)} for a rotation with one axis")
+        if tuple(ctx.positions.shape) != (ctx.rows,):
+            raise ValueError(f"AttentionBranch: positions {tuple(ctx.positions.shape)} for {ctx.rows} rows and a rotation with one axis")
         self.ctx = ctx
 
     @property

@@ -254,6 +254,9 @@ class _Layer:
         mk = lambda: torch.empty(rows, d.hidden, device=device, dtype=BF16)  # noqa: E731
         self.xn, self.mix, self.h1, self.y, self.part, self.out = mk(), mk(), mk(), mk(), mk(), mk()
 
+    def check(self, ctx) -> None:
+        """Raises ValueError where the layer cannot take ctx; called for every layer before the first one runs."""
+
     def mixer(self, x: torch.Tensor, ctx, mix: torch.Tensor) -> torch.Tensor:
         """Writes this rank's mixer contribution for all rows into mix and returns it already reduced."""
         raise NotImplementedError
@@ -388,19 +391,23 @@ class AttnLayer(_Layer):
         self._cu: dict[int, torch.Tensor] = {}
         self._ws: dict[int, tuple[int, torch.Tensor]] = {}
 
+    def check(self, ctx) -> None:
+        shape = tuple(ctx.positions.shape)
+        if self.axes is None:
+            if shape != (ctx.rows,):
+                raise ValueError(f"AttnLayer: positions {shape} for {ctx.rows} rows and a rotation with one axis")
+        elif shape not in ((ctx.rows,), (self.n_axes, ctx.rows)):
+            raise ValueError(f"AttnLayer: positions {shape} for {ctx.rows} rows and {self.n_axes} rotary axes")
+
     def _attend(self, x: torch.Tensor, ctx, out: torch.Tensor) -> torch.Tensor:
         """This rank's heads for the rows of x ([n, H], the rows of ctx): the o-projection into out [n, H]."""
         n, hd = x.shape[0], self.d.head_dim
         qkv = K.gemm(x, self.wqkv, out=self.qkv[:n])
         if self.axes is None:
-            if ctx.positions.dim() != 1:
-                raise ValueError(f"AttnLayer: positions {tuple(ctx.positions.shape)} for a rotation with one axis")
             K.qkv_rope_kv_write(qkv, self.nq, self.nkv, hd, ctx.positions, self.inv_freq, 1.0, self.q[:n], self.key_cache,
                                 self.value_cache, ctx.slot_mapping)
         else:
             pos = ctx.positions if ctx.positions.dim() == 2 else ctx.positions[None].expand(self.n_axes, -1)
-            if pos.shape[0] != self.n_axes:
-                raise ValueError(f"AttnLayer: positions {tuple(pos.shape)} for {self.n_axes} rotary axes")
             K.qkv_mrope_kv_write(qkv, self.nq, self.nkv, hd, pos, self.inv_freq, self.axes, 1.0, self.q[:n], self.key_cache,
                                  self.value_cache, ctx.slot_mapping)
         q, ao = self.q[:n].unflatten(1, (self.nq, hd)), self.ao[:n].unflatten(1, (self.nq, hd))
@@ -468,6 +475,8 @@ class Qwen35Stack:
         through every layer; returns the last layer's output buffer (valid until the next call)."""
         if h.shape[0] != ctx.rows:
             raise ValueError(f"Qwen35Stack.step: h has {h.shape[0]} rows, the context {ctx.rows}")
+        for layer in self.layers:
+            layer.check(ctx)
         for layer in self.layers:
             h = layer.step(h, ctx)
         return h

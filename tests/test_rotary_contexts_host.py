@@ -87,3 +87,26 @@ def test_one_axis_layer_refuses_several_axes_on_every_prefill(monkeypatch):
     with pytest.raises(ValueError, match="one axis"):
         layer.prefill(h, several)
     assert torch.equal(layer.prefill(h, pc), first)
+
+
+@pytest.mark.parametrize("sections", [(), (16, 8, 8)])
+def test_a_refused_step_leaves_the_states_as_they_were(monkeypatch, sections):
+    """Positions that the attention layer cannot take are found before the delta-rule layers ahead of it move their states."""
+    from multi_modal_parallelism_b200 import qwen35 as Q
+    from multi_modal_parallelism_b200.dist import Coordinator, Groups
+    from tests import _kernel_stand_ins as S
+
+    monkeypatch.setattr(Q, "K", S)
+    d = Q.Qwen35Dims(hidden=256, n_k=4, n_v=8, n_q=4, n_kv=2, head_dim=64, intermediate=256, layout="GA", rope_sections=sections)
+    g = Groups(rank=0, local_rank=0, world_size=1, tp=Coordinator((0,), None), pair=None, device=CPU)
+    pc = make_prefill_ctx([9, 6], 16, CPU)
+    stack = Q.Qwen35Stack(d, Q.random_stack(d, 0), "tp", g, CPU, 3, pc.block_table.numel(), 16, 40)
+    x = torch.randn(15, d.hidden, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16)
+    for ctx, n in ((pc, 15), (decode_ctx_after(pc), 2)):
+        for shape in [(n - 1,), (2 * n,), (3, n - 1), (2, n), (3, 2, n)] + ([] if sections else [(3, n)]):
+            with pytest.raises(ValueError, match="positions"):
+                stack.step(x[:n], dataclasses.replace(ctx, positions=torch.ones(shape, dtype=torch.int64)))
+    gdn = stack.layers[0]
+    assert not bool(gdn.ssm_state.any()) and not bool(gdn.conv_state.any())
+    stack.step(x, pc)
+    assert bool(gdn.ssm_state.any())
