@@ -38,7 +38,7 @@ struct MoeGroup {
   int place[16];
 };
 
-// Which kernels take a call. Up to 8 tokens one launch; then the few-token kernels while the second product is small (R places
+// Which kernels take a call. Up to 8 tokens and 64 places one launch; then the few-token kernels while the second product is small (R places
 // of I columns: its K dimension is I, at which the tensor-core kernels pay 128 columns and an accumulator's turn for each
 // expert), the tensor-core kernels else. Measured (us, few-token / tensor-core), H 2048 if not said:
 //   257 experts, I 64:  288 places 35 / 64, 1152 71 / 86;   I 128: 576 places 75 / 85, 1152 100 / 99

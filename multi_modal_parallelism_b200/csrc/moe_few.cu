@@ -10,7 +10,7 @@
 //   down: a block takes 16 columns of the output for ALL experts, its warps take (group, k range) tasks and leave 16 fp32
 //         a place in shared memory; then each token's places are summed in their order: no atomics, no partial results in
 //         HBM.
-// With at most 8 tokens the layer is one launch.
+// With at most 8 tokens and 64 places (7 tokens of 9) the layer is one launch.
 #include <algorithm>
 #include <cooperative_groups.h>
 

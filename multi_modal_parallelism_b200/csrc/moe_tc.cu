@@ -1,5 +1,5 @@
 // Mixture-of-experts products on the 5th-generation tensor cores (tcgen05 / TMEM / TMA), for more places than the few-token
-// kernels of moe.cu take: h = silu(x Wg_e^T) * (x Wu_e^T) and y = h Wd_e^T over sorted rows.
+// kernels of moe_few.cu take: h = silu(x Wg_e^T) * (x Wu_e^T) and y = h Wd_e^T over sorted rows.
 //
 // The weights are the 128-row M side of the MMA and the rows of one expert (a block of at most 256, as many as there are,
 // in steps of 16) its N side: an expert's weights are read once for up to 256 tokens and little of an MMA is padding. Up to

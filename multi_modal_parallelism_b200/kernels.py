@@ -846,7 +846,7 @@ def moe_experts(x: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, 
 def moe_layer(x: torch.Tensor, logits: torch.Tensor, w_gate_up: torch.Tensor, w_down: torch.Tensor, top_k: int,
               out: torch.Tensor | None = None, renormalize: bool = True, shared: bool = False,
               addend: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
-    """moe_route and moe_experts in one call, up to 8 tokens one launch. logits
+    """moe_route and moe_experts in one call, up to 8 tokens and 64 places (top_k, the shared one) one launch. logits
     [T, E] (shared: the same E columns, the last one the shared expert's gate; its weights are the last of w_gate_up and
     w_down)."""
     name = "moe_layer"
