@@ -461,7 +461,7 @@ class Qwen35Stack:
             raise ValueError(f"Qwen35Stack: mode {mode!r} not in {MODES}")
         if len(weights) != len(d.layout):
             raise ValueError(f"Qwen35Stack: {len(weights)} weight sets for layout {d.layout!r}")
-        self.d, self.mode, self.groups = d, mode, groups
+        self.d, self.mode, self.groups, self.max_tokens = d, mode, groups, max_tokens
         self.layers: list[_Layer] = []
         ws = _Moe.scratch(d, mlp_cols(d, groups.rank, groups.world_size), device, max_tokens) if d.n_experts else None
         for kind, w in zip(d.layout, weights):
@@ -475,6 +475,8 @@ class Qwen35Stack:
         through every layer; returns the last layer's output buffer (valid until the next call)."""
         if h.shape[0] != ctx.rows:
             raise ValueError(f"Qwen35Stack.step: h has {h.shape[0]} rows, the context {ctx.rows}")
+        if h.shape[0] > self.max_tokens:
+            raise ValueError(f"Qwen35Stack.step: {h.shape[0]} rows are more than max_tokens {self.max_tokens}")
         for layer in self.layers:
             layer.check(ctx)
         for layer in self.layers:
