@@ -39,7 +39,7 @@ def pytest_collection_modifyitems(config, items):
     if has_gpu:
         skip = pytest.mark.skip(reason="hands CPU tensors to the library: runs on a machine without a GPU")
         for it in items:
-            if it.nodeid.rpartition("/")[2].startswith(HOST_ONLY):
+            if f"{it.path.name}::{it.name}".startswith(HOST_ONLY):
                 it.add_marker(skip)
         return
     skip = pytest.mark.skip(reason="no CUDA device visible")
